@@ -103,6 +103,68 @@ void  trainlib_layernorm_fp16_bw_cl(void *trainlib_layernorm_args);
 void  trainlib_gelu_fp32_bw_cl(void *act_args);
 void  trainlib_gelu_fp16_bw_cl(void *act_args_fp16);
 
+/* ---- Feed-forward half of a transformer block beyond the reference, which has the norm of one vector, SwiGLU on its own and
+ * the matrix product [ref: lib/sources/pulp_rmsnorm_fp32.c:29-60, lib/sources/pulp_act_fp32.c:688-712].  Tensors are row-major and dense, a row per token; T is
+ * float for the fp32 entry points and fp16 for the fp16 ones.  Sums, statistics and scales are held in 32 bits.  The streams mode
+ * does not apply: `rows` counts every token.  Calls with rows or a size below 1, or without a pointer that they need, are refused
+ * (TL_ERR_BAD_ARGS) and touch nothing.  Host pointers are staged like everywhere; gradients are written, not accumulated.
+ *
+ * RMS norm of a residual sum.
+ *   fw:    h = x + residual (residual may be NULL: h = x);  output = weight * h / sqrt(mean(h^2) + eps) from the unrounded h;
+ *          sum, if not NULL, receives h.  sum or output may be x or residual itself.
+ *   int8:  the same, rounded to 8 bits with a scale for each row: q * scale = weight * h / sqrt(mean(h^2) + eps), scale = the row's
+ *          largest magnitude / 127, q rounded to nearest (ties to even).  A row of zeros has scale 0; a row whose result is not
+ *          finite has a scale that is not finite (q is 0 where a value is NaN).
+ *   bw:    `sum` is the input: the h that the forward pass left.  With r = 1 / sqrt(mean(h^2) + eps) and g = weight * dy:
+ *          dx = dsum + r * (g - h * r^2 * mean(g * h)) is the gradient of x and of residual; dsum (NULL: none) is the gradient that
+ *          reaches the sum along the residual path.  dweight[j] = sum over the rows of dy * h * r.  dx or dweight may be NULL (not
+ *          wanted), not both.  dx may be dy, dsum or sum itself.
+ * Every row is reduced in one fixed order and so are the rows of dweight: results are the same bits every time. */
+struct trainlib_rmsnorm_args {
+    void *x; void *residual; void *weight; void *sum; void *output;
+    signed char *q; float *scale;
+    float eps; int rows; int size;
+    void *dy; void *dsum; void *dx; void *dweight;
+};
+void  trainlib_rmsnorm_fp32_fw_cl(void *trainlib_rmsnorm_args);
+void  trainlib_rmsnorm_fp16_fw_cl(void *trainlib_rmsnorm_args);
+void  trainlib_rmsnorm_int8_fp32_fw_cl(void *trainlib_rmsnorm_args);
+void  trainlib_rmsnorm_int8_fp16_fw_cl(void *trainlib_rmsnorm_args);
+void  trainlib_rmsnorm_fp32_bw_cl(void *trainlib_rmsnorm_args);
+void  trainlib_rmsnorm_fp16_bw_cl(void *trainlib_rmsnorm_args);
+
+/* Gated feed-forward block: gate = x Wg^T, up = x Wu^T, y = (silu(gate) * up) Wd^T with silu(v) = v / (1 + exp(-v)).
+ * x [rows][in_size], w_gate and w_up [hidden][in_size], w_down [out_size][hidden], gate and up [rows][hidden], y [rows][out_size].
+ *   fw:  reads x and the weights, writes y; gate and up, both or neither, receive the projections for a backward pass.
+ *   bw:  reads dy, gate and up (as the forward pass left them) and what the wanted gradients need: w_down for dx, dw_gate and
+ *        dw_up; w_gate and w_up for dx; x for dw_gate and dw_up.  Any of dx, dw_gate, dw_up, dw_down may be NULL (not wanted), not all.
+ * The product silu(gate) * up and its gradients are library scratch of `rows * hidden` elements each: three of them in the backward
+ * pass.  In fp16 they are rounded to fp16 between the products (what passes 65504 there is infinite).  Outputs must not overlap inputs. */
+struct trainlib_gated_ffn_args {
+    void *x; void *w_gate; void *w_up; void *w_down; void *gate; void *up; void *y;
+    int rows; int in_size; int hidden; int out_size;
+    void *dy; void *dx; void *dw_gate; void *dw_up; void *dw_down;
+};
+void  trainlib_gated_ffn_fp32_fw_cl(void *trainlib_gated_ffn_args);
+void  trainlib_gated_ffn_fp16_fw_cl(void *trainlib_gated_ffn_args);
+void  trainlib_gated_ffn_fp32_bw_cl(void *trainlib_gated_ffn_args);
+void  trainlib_gated_ffn_fp16_bw_cl(void *trainlib_gated_ffn_args);
+
+/* Linear layer in 8 bits: y[r][o] = x_scale[r] * w_scale[o] * sum_i x[r][i] * weight[o][i] (+ bias[o]); x [rows][in_size], weight
+ * [out_size][in_size] (as Linear_args has it), y and bias (may be NULL) of type T.  The sums are exact in 32-bit integers, for which
+ * in_size may be at most 131071 (TL_ERR_TOO_LARGE beyond).  y must not overlap the inputs.
+ * trainlib_quantize_rows: the 8-bit form of a tensor's rows, of a layer's tokens or (once) of its weights' channels:
+ * scale[r] = max_i |x[r][i]| / 127, q = x / scale rounded to nearest (ties to even); zeros and what is not finite as for the norm. */
+struct trainlib_linear_int8_args {
+    signed char *x; float *x_scale; signed char *weight; float *w_scale; void *bias; void *y;
+    int rows; int in_size; int out_size;
+};
+void  trainlib_linear_int8_fp32_fw_cl(void *trainlib_linear_int8_args);
+void  trainlib_linear_int8_fp16_fw_cl(void *trainlib_linear_int8_args);
+struct trainlib_quantize_rows_args { void *x; signed char *q; float *scale; int rows; int size; };
+void  trainlib_quantize_rows_fp32_cl(void *trainlib_quantize_rows_args);
+void  trainlib_quantize_rows_fp16_cl(void *trainlib_quantize_rows_args);
+
 /* ---- Instance norm fused with what follows it in a residual network.  No counterpart in the reference, which runs
  * pulp_instnorm_*_fw_cl, pulp_residualconn_*_fw and pulp_relu_*_fw_cl one after the other
  * (lib/sources/pulp_instnorm_fp32.c:27, pulp_residual_fp32.c:26, pulp_act_fp32.c:83); results are those of that sequence,

@@ -11,7 +11,7 @@ import os
 import numpy as np
 
 from . import abi
-from .abi import STRUCTS, FUNCTIONS, addr
+from .abi import STRUCTS, FUNCTIONS, EXT_FUNCTIONS, EXT_STRUCTS, addr
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtrainlib_b200.so")
@@ -45,7 +45,7 @@ def load(path=LIB_PATH):
     if not os.path.exists(path):
         raise RuntimeError("%s not found: build it with `make -C %s` (or __graft_entry__.build())"
                            % (path, os.path.join(_HERE, "csrc")))
-    lib = bind(ctypes.CDLL(path))
+    lib = bind(bind(ctypes.CDLL(path)), EXT_FUNCTIONS)
     lib.trainlib_init.argtypes = [ctypes.c_int]; lib.trainlib_init.restype = ctypes.c_int
     lib.trainlib_last_error.restype = ctypes.c_int
     lib.trainlib_last_error_string.restype = ctypes.c_char_p
@@ -121,9 +121,9 @@ def make_blob(keep, data=None, diff=None, C=1, H=1, W=1, dim=None, half=False):
 
 
 def make_args(keep, struct_name, **fields):
-    """Fill one of the reference's argument structs; pointer fields accept structs, arrays, ints."""
-    s = STRUCTS[struct_name]()
-    kinds = dict(abi.STRUCT_FIELDS[struct_name])
+    """Fill one of the reference's argument structs, or one of the extensions'; pointer fields accept structs, arrays, ints."""
+    s = (STRUCTS.get(struct_name) or EXT_STRUCTS[struct_name])()
+    kinds = dict(abi.STRUCT_FIELDS.get(struct_name) or abi.EXT_STRUCT_FIELDS[struct_name])
     for k, v in fields.items():
         if k not in kinds:
             raise KeyError("%s has no field %s" % (struct_name, k))

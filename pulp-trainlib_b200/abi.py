@@ -13,6 +13,7 @@ import os
 import re
 
 HEADER = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "include", "trainlib_b200_abi.h")
+EXT_HEADER = os.path.join(os.path.dirname(HEADER), "trainlib_b200.h")          # the extensions' structs and entry points
 
 _SCALARS = {"float": ctypes.c_float, "int": ctypes.c_int, "fp16": ctypes.c_uint16}
 
@@ -61,6 +62,9 @@ def _make(name, fields):
 
 
 STRUCTS = {name: _make(name, fields) for name, fields in STRUCT_FIELDS.items()}
+EXT_STRUCT_FIELDS = parse_structs(EXT_HEADER)
+EXT_STRUCTS = {name: _make(name, fields) for name, fields in EXT_STRUCT_FIELDS.items()}
+EXT_FUNCTIONS = [name for name in parse_functions(EXT_HEADER) if name.endswith("_cl")]
 globals().update(STRUCTS)
 
 

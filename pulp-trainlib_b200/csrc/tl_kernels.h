@@ -234,6 +234,21 @@ template <class T> void sm_bw_op2(const T *A, const T *B, const T *S, T *out, in
 void cast_h2f(const __half *src, float *dst, long long n);
 void cast_f2h(const float *src, __half *dst, long long n);
 
+// ---------------------------------------------------------------- feed-forward half of a transformer block
+template <class T> void rmsnorm_fw(const T *x, const T *res, const T *w, T *sum, T *y, int rows, int size, float eps);
+template <class T> void rmsnorm_int8_fw(const T *x, const T *res, const T *w, T *sum, signed char *q, float *scale, int rows, int size, float eps);
+template <class T> void rmsnorm_bw(Scope &sc, const T *h, const T *w, const T *dy, const T *dsum, T *dx, T *dw, int rows, int size, float eps);
+template <class T> void quantize_rows(const T *x, signed char *q, float *scale, int rows, int size);
+template <class T> void linear_int8(Scope &sc, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out);
+// null: not wanted (forward: g and u; backward: any gradient)
+template <class T> struct GatedFfn {
+    const T *x, *wg, *wu, *wd, *dy;
+    T *g, *u, *y, *dx, *dwg, *dwu, *dwd;
+    int rows, in, hidden, out;
+};
+template <class T> void gated_ffn_fw(Scope &sc, const GatedFfn<T> &f);
+template <class T> void gated_ffn_bw(Scope &sc, const GatedFfn<T> &f);
+
 // ---------------------------------------------------------------- attention
 struct MhsaDims { int L, E, F, heads; };
 struct MobileBertDims { int L, E, Kb, F, No, heads; };
