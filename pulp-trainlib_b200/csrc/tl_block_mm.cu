@@ -1,0 +1,612 @@
+// The products of the feed-forward block and of the 8-bit linear layer on the tensor cores (tcgen05, operands by TMA, accumulators in tensor memory).
+// Persistent CTAs walk tiles of 128 rows (256 for a CTA pair) x BN accumulator columns: a producer warp fills a ring of shared-memory
+// stages of 128 bytes of K per row, an issuer warp multiplies them, eight warps take finished accumulators out and apply the epilogue.
+//   gate:      the B operand of a tile is BN / 2 rows of Wg and the same rows of Wu (in a pair: one CTA's shared memory holds Wg's, the
+//              other's Wu's), so that gate and up of a result lie BN / 2 columns apart in the same lane: H, and if wanted G and U, leave from
+//              registers and the pre-activations are never read back.
+//   gate, bw:  dH stays in the accumulator; the epilogue reads G and U and writes H, dG and dU.
+//   8 bits:    kind::i8, 32-bit integer accumulators (exact); scales and bias in the epilogue.
+//   fp32:      3xTF32 on packed (hi, lo) pairs: D0 = A_hi [B_hi | B_lo]^T, D1 = A_lo B_hi^T.  The accumulator truncates: each step takes up to 2^-23 of it
+//              off towards zero, which over a chain of n steps is 0.24 n 2^-23 of the result (4e-6 at K = 1024).  So every 128 of K
+//              the accumulators are added to sums in registers, rounded to nearest, and started anew: 5e-7 at any K.
+// Few tiles: `splits` CTAs share a tile's K and leave partial tiles, which bm_reduce_kernel adds in order (with the same epilogue).
+// No multicast loads.  Every wait is bounded and reports through the status word.
+#include "tl_tma_mm.cuh"
+#include "tl_gate.cuh"
+#include <algorithm>
+
+namespace tl {
+
+enum { MM_F16 = 0, MM_TF32 = 1, MM_I8 = 2 };
+static constexpr int BM_ROWS = 128, BM_EPI = 8, BM_THREADS = 32 * (BM_EPI + 2), BM_MAX_STAGES = 8;
+static constexpr uint32_t BM_RING = 200 * 1024;
+static constexpr int BM_CHUNK = 4;                     // fp32: K steps of 32 between two drains of the accumulators
+
+template <int KIND> struct BmCfg { static constexpr int BK = KIND == MM_F16 ? 64 : KIND == MM_TF32 ? 32 : 128, PARTS = KIND == MM_TF32 ? 2 : 1; };
+
+template <class T> struct BmParams {
+    T *C, *g, *u, *dg, *du;
+    const T *bias; const float *xs, *ws;
+    uint32_t *part;
+    int N, M, tiles_m, tiles_n, tiles, kps, ksteps, splits, stages, a_mn, b_mn, vec;       // kps: K steps of a term
+    uint32_t stage_bytes;
+    int *status;
+};
+struct BmMaps { CUtensorMap a[2], b[2]; };
+
+// D = A B^T of 8-bit integers, 32 bytes of K
+template <bool PAIR> __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// accumulators of 32-bit integers (2), operands of signed 8 bits (1), both K-major
+__host__ __device__ constexpr uint32_t i8_idesc(uint32_t M, uint32_t N) { return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24); }
+
+// ---------------------------------------------------------------- epilogue of W neighbouring results of a row
+template <int W> __device__ __forceinline__ void bm_st(float *p, const float (&v)[W], int live, bool vec)
+{
+    if (vec && live >= W) {
+#pragma unroll
+        for (int j = 0; j < W; j += 4) *reinterpret_cast<float4 *>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; j++) if (j < live) p[j] = v[j];
+    }
+}
+__device__ __forceinline__ uint32_t bm_half2(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <int W> __device__ __forceinline__ void bm_st(__half *p, const float (&v)[W], int live, bool vec)
+{
+    if (vec && live >= W) {
+        if constexpr (W % 8 == 0) {
+#pragma unroll
+            for (int j = 0; j < W; j += 8)
+                *reinterpret_cast<uint4 *>(p + j) = make_uint4(bm_half2(v[j], v[j + 1]), bm_half2(v[j + 2], v[j + 3]), bm_half2(v[j + 4], v[j + 5]), bm_half2(v[j + 6], v[j + 7]));
+        } else *reinterpret_cast<uint2 *>(p) = make_uint2(bm_half2(v[0], v[1]), bm_half2(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; j++) if (j < live) st(p + j, v[j]);
+    }
+}
+template <int W> __device__ __forceinline__ void bm_ld(const float *p, float (&v)[W], int live, bool vec)
+{
+    if (vec && live >= W) {
+#pragma unroll
+        for (int j = 0; j < W; j += 4) { const float4 x = *reinterpret_cast<const float4 *>(p + j); v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w; }
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; j++) v[j] = ld0(j < live, p + j);
+    }
+}
+__device__ __forceinline__ void bm_unpack(uint32_t w, float &a, float &b)
+{
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    a = f.x; b = f.y;
+}
+template <int W> __device__ __forceinline__ void bm_ld(const __half *p, float (&v)[W], int live, bool vec)
+{
+    if (vec && live >= W) {
+        if constexpr (W % 8 == 0) {
+#pragma unroll
+            for (int j = 0; j < W; j += 8) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(p + j);
+                bm_unpack(x.x, v[j], v[j + 1]); bm_unpack(x.y, v[j + 2], v[j + 3]); bm_unpack(x.z, v[j + 4], v[j + 5]); bm_unpack(x.w, v[j + 6], v[j + 7]);
+            }
+        } else { const uint2 x = *reinterpret_cast<const uint2 *>(p); bm_unpack(x.x, v[0], v[1]); bm_unpack(x.y, v[2], v[3]); }
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; j++) v[j] = ld0(j < live, p + j);
+    }
+}
+// v: the accumulators (gate), w: the second ones (up); row and col are inside the result
+template <class T, int EPI, int W> __device__ __forceinline__ void bm_results(const BmParams<T> &p, int row, int col, float (&v)[W], float (&w)[W])
+{
+    constexpr bool FAST = sizeof(T) == 2;
+    const size_t at = (size_t)row * p.M + col;
+    const int live = p.M - col;
+    if constexpr (EPI == FFN_GATE) {
+        if (p.g) { bm_st<W>(p.g + at, v, live, p.vec); bm_st<W>(p.u + at, w, live, p.vec); }
+#pragma unroll
+        for (int j = 0; j < W; j++) v[j] = gate_fw<FAST>(v[j], w[j]);
+    } else if constexpr (EPI == FFN_GATE_BW) {
+        float g[W], u[W];
+        bm_ld<W>(p.g + at, g, live, p.vec); bm_ld<W>(p.u + at, u, live, p.vec);
+#pragma unroll
+        for (int j = 0; j < W; j++) { const float dh = v[j]; gate_bw<FAST>(g[j], u[j], dh, v[j], g[j], u[j]); }
+        bm_st<W>(p.dg + at, g, live, p.vec); bm_st<W>(p.du + at, u, live, p.vec);
+    } else if constexpr (EPI == FFN_INT8) {
+        const float xs = p.xs[row];
+#pragma unroll
+        for (int j = 0; j < W; j++) v[j] = v[j] * xs * ld0(j < live, p.ws + col + j) + ld0(p.bias && j < live, p.bias + col + j);
+    }
+    bm_st<W>(p.C + at, v, live, p.vec);
+}
+
+// tile -> row block, column block: eight row blocks share a sweep over the columns
+template <class T> __device__ __forceinline__ void bm_locate(const BmParams<T> &p, int tile, int &rb, int &cb)
+{
+    const int g = tile / (8 * p.tiles_m), in = tile - g * 8 * p.tiles_m, rows = min(8, p.tiles_n - 8 * g);
+    rb = 8 * g + in % rows; cb = in / rows;
+}
+
+template <int KIND, class T, int EPI, int BN, bool PAIR>
+__global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_constant__ BmMaps maps, const __grid_constant__ BmParams<T> p)
+{
+    pdl_wait();
+    constexpr int BK = BmCfg<KIND>::BK, PARTS = BmCfg<KIND>::PARTS;
+    constexpr int BNL = PAIR ? BN / 2 : BN;                                         // rows of B in this CTA's shared memory
+    constexpr int BNC = EPI == FFN_GATE ? BN / 2 : BN;                              // result columns of a tile
+    constexpr int CW = BNC / 2;                                                     // of a warp
+    constexpr int ROWS = PAIR ? 2 * BM_ROWS : BM_ROWS;
+    constexpr uint32_t A_BYTES = BM_ROWS * 128u, B_BYTES = BNL * 128u;
+    constexpr int NBUF = KIND == MM_TF32 && BN > 64 ? 1 : 2;
+    constexpr uint32_t BUF_COLS = 256;
+    extern __shared__ unsigned char bsm_raw[];
+    const uint32_t sbase = (smem_u32(bsm_raw) + 1023u) & ~1023u;                    // swizzle atoms want 1024-byte alignment
+    __shared__ uint64_t full[BM_MAX_STAGES], empty[BM_MAX_STAGES], acc_full[2], acc_empty[2], last_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int failed_s;
+    volatile int *failed = &failed_s;
+
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int ST = p.stages;
+    const int group = PAIR ? 2 : p.splits, rank = (int)blockIdx.x % group, first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
+    const int ks0 = PAIR ? 0 : p.ksteps * rank / p.splits, ks1 = PAIR ? p.ksteps : p.ksteps * (rank + 1) / p.splits;
+    const int row_of_tile = PAIR ? rank * BM_ROWS : 0;
+
+    if (tid == 0) {
+        for (int s = 0; s < ST; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; b++) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], PAIR ? 2 * BM_EPI : BM_EPI); }
+        mbar_init(&last_bar, 1);
+        failed_s = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&maps.a[0]); tma_prefetch_desc(&maps.b[0]);
+    }
+    if (warp == 0) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
+    }
+    tc_fence_before();
+    if constexpr (PAIR) tm_cluster_sync();                                          // the other CTA's barriers are initialised too
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    if (warp == BM_EPI) {
+        // producer (whole warp; a thread is elected around the instructions)
+        const uint32_t full0 = PAIR ? tm_mapa(smem_u32(&full[0]), 0) : 0u;          // the pair's leader counts both CTAs' bytes
+        int s = 0;
+        uint32_t phase = 1, issued = 0;                                             // the first pass over the ring finds it empty
+        bool ok = true;
+        for (int tile = first; tile < p.tiles && ok; tile += step) {
+            int rb, cb;
+            bm_locate(p, tile, rb, cb);
+            const int row0 = rb * ROWS + row_of_tile, col0 = cb * BNC;
+            int term = ks0 / p.kps, kt = ks0 - term * p.kps;
+            for (int k = ks0; k < ks1; k++) {
+                if (!tm_wait(&empty[s], phase, failed)) { ok = false; break; }
+                if (elect_one()) {
+                    const uint32_t st = sbase + s * p.stage_bytes, sb = st + PARTS * A_BYTES;
+                    const uint32_t bar = full0 + 8u * s;
+                    auto load = [&](uint32_t dst, const CUtensorMap *m, int x, int y, int z) {
+                        if constexpr (PAIR) tma_load_3d_pair(dst, m, bar, x, y, z);
+                        else tma_load_3d(dst, m, &full[s], x, y, z);
+                    };
+                    if (!PAIR || rank == 0) mbar_arrive_expect_tx(&full[s], PAIR ? 2 * p.stage_bytes : p.stage_bytes);
+                    const CUtensorMap *ma = &maps.a[term], *mb = &maps.b[EPI == FFN_GATE ? 0 : term];
+#pragma unroll
+                    for (int z = 0; z < PARTS; z++) {
+                        if (KIND == MM_F16 && p.a_mn) { for (int j = 0; j < 2; j++) load(st + j * 8192u, ma, row0 + 64 * j, kt * BK, 0); }
+                        else load(st + z * A_BYTES, ma, kt * BK, row0, z);
+                        if constexpr (EPI == FFN_GATE) {
+                            if constexpr (PAIR) load(sb, &maps.b[rank], kt * BK, col0, 0);
+                            else {
+                                load(sb + z * B_BYTES, &maps.b[0], kt * BK, col0, z);
+                                load(sb + z * B_BYTES + B_BYTES / 2, &maps.b[1], kt * BK, col0, z);
+                            }
+                        } else {
+                            const int c = col0 + (PAIR ? rank * BNL : 0);
+                            if (KIND == MM_F16 && p.b_mn) { for (int j = 0; j < BNL / 64; j++) load(sb + j * 8192u, mb, c + 64 * j, kt * BK, 0); }
+                            else load(sb + z * B_BYTES, mb, kt * BK, c, z);
+                        }
+                    }
+                }
+                __syncwarp();
+                issued++;
+                if (++kt == p.kps) { kt = 0; term++; }
+                if (++s == ST) { s = 0; phase ^= 1u; }
+            }
+        }
+        // given up: the copies still under way land before the shared memory is left (the pair's leader sees both CTAs')
+        if (!ok && (!PAIR || rank == 0))
+            for (int j = 0; j < ST; j++) {
+                if ((uint32_t)j >= issued && issued < (uint32_t)ST) break;
+                const uint32_t parity = j < s ? phase ^ 1u : phase;
+                for (int i = 0; i < 100000 && !mbar_try_wait(&full[j], parity); i++) __nanosleep(100);
+            }
+    } else if (warp == BM_EPI + 1) {
+        if (!PAIR || rank == 0) {
+            const uint32_t majors = (p.a_mn ? IDESC_A_MN_MAJOR : 0u) | (p.b_mn ? IDESC_B_MN_MAJOR : 0u);
+            const uint32_t idesc = KIND == MM_F16 ? (mma_idesc(FMT_F16, ROWS, BN) | majors) : KIND == MM_I8 ? i8_idesc(ROWS, BN) : mma_idesc(FMT_TF32, ROWS, 2 * BN);
+            const uint32_t idesc_lo = mma_idesc(FMT_TF32, ROWS, BN);
+            // descriptor words that do not depend on the stage, and the step of one MMA (32 bytes or 16 rows of K) in 16-byte units
+            const uint64_t desc_a = KIND == MM_F16 && p.a_mn ? smem_desc_swizzled(0, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(0, 1024);
+            const uint64_t desc_b = KIND == MM_F16 && p.b_mn ? smem_desc_swizzled(0, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(0, 1024);
+            const uint32_t step_a = KIND == MM_F16 && p.a_mn ? 128u : 2u, step_b = KIND == MM_F16 && p.b_mn ? 128u : 2u;
+            int s = 0, it = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = first; tile < p.tiles && ok; tile += step)
+                for (int kc = ks0; kc < ks1 && ok; it++) {
+                    const int kend = KIND == MM_TF32 ? min(ks1, kc + BM_CHUNK) : ks1, buf = it % NBUF, use = it / NBUF;
+                    if (use > 0 && !tm_wait(&acc_empty[buf], (uint32_t)(use - 1) & 1u, failed)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t d = tmem + buf * BUF_COLS;
+                    uint32_t acc = 0;
+                    for (; kc < kend; kc++) {
+                        if (!tm_wait(&full[s], phase, failed)) { ok = false; break; }
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t st = sbase + s * p.stage_bytes, sb = st + PARTS * A_BYTES;
+                            const uint64_t da = desc_a + (st >> 4), db = desc_b + (sb >> 4);
+#pragma unroll
+                            for (int kk = 0; kk < 4; kk++) {                        // 4 MMAs of 32 bytes of K each per 128-byte row
+                                if constexpr (KIND == MM_I8) mma_i8<PAIR>(d, da + kk * step_a, db + kk * step_b, idesc, kk ? 1u : acc);
+                                else tm_mma<KIND == MM_F16, PAIR>(d, da + kk * step_a, db + kk * step_b, idesc, kk ? 1u : acc);
+                                if constexpr (KIND == MM_TF32) tm_mma<false, PAIR>(d + 2 * BN, da + (A_BYTES >> 4) + kk * step_a, db + kk * step_b, idesc_lo, kk ? 1u : acc);
+                            }
+                            tm_commit<PAIR>(&empty[s]);
+                        }
+                        __syncwarp();
+                        acc = 1u;
+                        if (++s == ST) { s = 0; phase ^= 1u; }
+                    }
+                    if (ok && elect_one()) tm_commit<PAIR>(&acc_full[buf]);
+                    __syncwarp();
+                }
+            if (!ok) {                                                              // given up: what was issued ends first
+                if (elect_one()) tm_commit<PAIR>(&last_bar);
+                __syncwarp();
+                for (int i = 0; i < 100000 && !mbar_try_wait(&last_bar, 0); i++) __nanosleep(100);
+            }
+        }
+    } else {
+        // epilogue: warp w owns TMEM lanes 32 (w % 4) .. + 31, one row each, and one half of the tile's result columns
+        const int quarter = warp & 3, half = warp >> 2;
+        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+        const int row_in = quarter * 32 + lane;
+        int it = 0;
+        bool ok = true;
+        for (int tile = first; tile < p.tiles && ok; tile += step) {
+            int rb, cb;
+            bm_locate(p, tile, rb, cb);
+            const int row = rb * ROWS + row_of_tile + row_in, col0 = cb * BNC + half * CW;
+            constexpr int NS = KIND == MM_TF32 ? CW : 1, NS2 = KIND == MM_TF32 && EPI == FFN_GATE ? CW : 1;
+            float sum[NS], sum2[NS2];
+            auto take = [&](uint32_t d, int c, float (&v)[16]) {                    // 16 accumulators of this lane's row
+                uint32_t a[16];
+                tmem_ld16(d + c, a);
+                if constexpr (KIND == MM_TF32) {
+                    uint32_t b[16], x[16];
+                    tmem_ld16(d + BN + c, b); tmem_ld16(d + 2 * BN + c, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = __uint_as_float(a[j]) + (__uint_as_float(b[j]) + __uint_as_float(x[j]));
+                } else {
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = KIND == MM_I8 && p.splits == 1 ? (float)(int)a[j] : __uint_as_float(a[j]);
+                }
+            };
+            auto release = [&](int buf) {                                           // the accumulators are in registers: they may be overwritten
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) { if constexpr (PAIR) tm_arrive_at(tm_mapa(smem_u32(&acc_empty[buf]), 0)); else mbar_arrive(&acc_empty[buf]); }
+            };
+            auto arrived = [&](int buf, int use) {
+                bool there = true;
+                if (lane == 0) there = tm_wait(&acc_full[buf], (uint32_t)use & 1u, failed, 32);
+                there = __shfl_sync(0xffffffffu, there ? 1 : 0, 0) != 0;
+                tc_fence_after();
+                return there;
+            };
+            uint32_t *mine = p.part + ((size_t)(tile * p.splits + rank) * BM_ROWS + row_in) * BN;        // row of the partial tile (splits > 1)
+            auto leave = [&](int c, float (&v)[16], float (&w)[16]) {
+                if (!PAIR && p.splits > 1) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        *reinterpret_cast<float4 *>(mine + half * CW + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        if constexpr (EPI == FFN_GATE) *reinterpret_cast<float4 *>(mine + BNC + half * CW + c + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+                    }
+                } else if (row < p.N && col0 + c < p.M) bm_results<T, EPI, 16>(p, row, col0 + c, v, w);
+            };
+            if constexpr (KIND == MM_TF32) {
+#pragma unroll
+                for (int j = 0; j < NS; j++) sum[j] = 0.f;
+#pragma unroll
+                for (int j = 0; j < NS2; j++) sum2[j] = 0.f;
+                for (int kc = ks0; kc < ks1; kc += BM_CHUNK, it++) {
+                    const int buf = it % NBUF, use = it / NBUF;
+                    if (!arrived(buf, use)) { ok = false; break; }
+                    const uint32_t d = tmem + lane_addr + buf * BUF_COLS;
+#pragma unroll
+                    for (int c = 0; c < CW; c += 16) {
+                        float v[16];
+                        take(d, half * CW + c, v);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) sum[c + j] += v[j];
+                        if constexpr (EPI == FFN_GATE) {
+                            take(d, BNC + half * CW + c, v);
+#pragma unroll
+                            for (int j = 0; j < 16; j++) sum2[c + j] += v[j];
+                        }
+                    }
+                    release(buf);
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int c = 0; c < CW; c += 16) {
+                    float v[16], w[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) { v[j] = sum[c + j]; w[j] = EPI == FFN_GATE ? sum2[EPI == FFN_GATE ? c + j : 0] : 0.f; }
+                    leave(c, v, w);
+                }
+            } else {
+                const int buf = it % NBUF, use = it / NBUF;
+                it++;
+                if (!arrived(buf, use)) { ok = false; break; }
+                const uint32_t d = tmem + lane_addr + buf * BUF_COLS;
+#pragma unroll 1
+                for (int c = 0; c < CW; c += 16) {
+                    float v[16], w[16];
+                    take(d, half * CW + c, v);
+                    if constexpr (EPI == FFN_GATE) take(d, BNC + half * CW + c, w);
+                    if (c + 16 >= CW) release(buf);
+                    leave(c, v, w);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*failed && tid == 0) atomicCAS(p.status, 0, 9);
+    if constexpr (PAIR) {
+        tm_cluster_sync();                                                          // both CTAs are done with each other's memory
+        if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        tm_cluster_sync();
+    } else if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// four neighbouring sums over the partial tiles: whole numbers as such
+template <int KIND, int BN> __device__ __forceinline__ void bm_add_parts(const uint32_t *from, int splits, float (&t)[4])
+{
+    if constexpr (KIND == MM_I8) {
+        int n[4] = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int k = 0; k < splits; k++) { const int4 x = *reinterpret_cast<const int4 *>(from + (size_t)k * BM_ROWS * BN); n[0] += x.x; n[1] += x.y; n[2] += x.z; n[3] += x.w; }
+#pragma unroll
+        for (int j = 0; j < 4; j++) t[j] = (float)n[j];
+    } else {
+        t[0] = t[1] = t[2] = t[3] = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < splits; k++) { const float4 x = *reinterpret_cast<const float4 *>(from + (size_t)k * BM_ROWS * BN); t[0] += x.x; t[1] += x.y; t[2] += x.z; t[3] += x.w; }
+    }
+}
+// The results from the partial tiles of a split contraction: a thread per four neighbouring results, partial tiles added in order.
+template <int KIND, class T, int EPI, int BN> __global__ void __launch_bounds__(256) bm_reduce_kernel(const __grid_constant__ BmParams<T> p)
+{
+    pdl_wait();
+    constexpr int BNC = EPI == FFN_GATE ? BN / 2 : BN, QUADS = BNC / 4, PER = BM_ROWS * QUADS;       // (PER is a multiple of 256: a block stays inside one tile)
+    const int e = blockIdx.x * 256 + threadIdx.x, tile = e / PER, in = e - tile * PER, r = in / QUADS, c = (in - r * QUADS) * 4;
+    int rb, cb;
+    bm_locate(p, tile, rb, cb);
+    const int row = rb * BM_ROWS + r, col = cb * BNC + c;
+    if (row >= p.N || col >= p.M) return;
+    const uint32_t *src = p.part + ((size_t)tile * p.splits * BM_ROWS + r) * BN + c;
+    float v[4], w[4];
+    bm_add_parts<KIND, BN>(src, p.splits, v);
+    if constexpr (EPI == FFN_GATE) bm_add_parts<KIND, BN>(src + BNC, p.splits, w);
+    bm_results<T, EPI, 4>(p, row, col, v, w);
+}
+
+// ---------------------------------------------------------------- launch
+static bool bm_map(CUtensorMap *m, CUtensorMapDataType type, int esize, const void *base, int inner, int outer, int parts, long long os, long long ps, int box_inner, int box_outer)
+{
+    EncodeTiledFn enc = (EncodeTiledFn)tc_encode_tiled_fn();
+    cuuint64_t gdim[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)parts};
+    cuuint64_t gstr[2] = {(cuuint64_t)(os * esize), (cuuint64_t)((parts > 1 ? ps : (long long)outer * os) * esize)};
+    cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1u}, estr[3] = {1, 1, 1};
+    return enc && enc(m, type, 3, (void *)base, gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Tile and CTAs per tile with the fewest cycles by the model that the plain products use (tl_gemm_tma.cu): a K step costs its tensor time or
+// what its bytes take from L2 into an SM (58 bytes per cycle with every SM loading, 81 with half of them), a pair's a third more than its tensor
+// time; a tile 2500 cycles beside its K steps, a launch 2000 (pairs 10000), partial tiles a launch and their bytes.
+struct BmPlan { int BN, pair, splits; };
+static BmPlan bm_plan(int kind, int epi, int N, int M, int ksteps)
+{
+    BmPlan plan = {64, 0, 1};
+    double best = 1e30;
+    const int bns[4] = {256, 128, 64, 256};
+    for (int i = kind == MM_TF32 ? 1 : 0; i < (kind == MM_TF32 ? 3 : 4); i++) {
+        const bool two = i == 3;
+        const int bn = bns[i], bnc = epi == FFN_GATE ? bn / 2 : bn;
+        const long long tiles = (long long)ceil_div(N, two ? 256 : 128) * ceil_div(M, bnc);
+        for (int s = 1; s <= (two ? 1 : 16); s++) {
+            if (s > 1 && (ksteps < 2 * s || tiles * s > sm_count())) break;
+            const long long ctas = tiles * s * (two ? 2 : 1);
+            const double tensor = (kind == MM_TF32 ? 6.0 : 2.0) * bn * (two ? 4.0 / 3.0 : 1.0);
+            const double fill = (kind == MM_TF32 ? 2 : 1) * 128.0 * (128 + (two ? bn / 2 : bn)) / (ctas <= sm_count() / 2 ? 81.0 : 58.0);
+            const double reduce = s > 1 ? 4000.0 + 512.0 * bn * tiles * s / 2000.0 : 0.0;
+            const double cost = (two ? 10000.0 : 2000.0) + (double)ceil_div(ctas, sm_count()) * (std::max(tensor, fill) * ceil_div(ksteps, s) + 2500.0) + reduce;
+            if (cost < 0.97 * best) { best = cost; plan = {bn, two ? 1 : 0, s}; }
+        }
+    }
+    return plan;
+}
+
+template <int KIND, class T, int EPI, int BN, bool PAIR> static void bm_launch(const BmMaps &maps, const BmParams<T> &p)
+{
+    const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
+    static bool attr_set = false;
+    if (!attr_set) {
+        cudaFuncSetAttribute(block_mm_kernel<KIND, T, EPI, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(BM_RING + 1024));
+        attr_set = true;
+    }
+    if constexpr (PAIR) TL_LAUNCH_CLUSTER((block_mm_kernel<KIND, T, EPI, BN, PAIR>), (unsigned)(2 * std::min(p.tiles, sm_count() / 2)), BM_THREADS, smem, 2, maps, p);
+    else {
+        TL_LAUNCH((block_mm_kernel<KIND, T, EPI, BN, PAIR>), (unsigned)(p.splits > 1 ? p.tiles * p.splits : std::min(p.tiles, sm_count())), BM_THREADS, smem, maps, p);
+        if (p.splits > 1) TL_LAUNCH((bm_reduce_kernel<KIND, T, EPI, BN>), (unsigned)((long long)p.tiles * BM_ROWS * (EPI == FFN_GATE ? BN / 2 : BN) / 4 / 256), 256, 0, p);
+    }
+}
+template <int KIND, class T, int EPI> static void bm_dispatch(const BmPlan &plan, const BmMaps &maps, const BmParams<T> &p)
+{
+    if constexpr (KIND != MM_TF32) {
+        if (plan.pair) return bm_launch<KIND, T, EPI, 256, true>(maps, p);
+        if (plan.BN == 256) return bm_launch<KIND, T, EPI, 256, false>(maps, p);
+    }
+    if (plan.BN == 128) bm_launch<KIND, T, EPI, 128, false>(maps, p);
+    else bm_launch<KIND, T, EPI, 64, false>(maps, p);
+}
+// what does not depend on the operands' layout; false: no memory for the partial tiles
+template <int KIND, class T, int EPI> static bool bm_setup(Scope &sc, const BmPlan &plan, BmParams<T> &p)
+{
+    const int bnc = EPI == FFN_GATE ? plan.BN / 2 : plan.BN;
+    p.status = tc_status_word();
+    p.splits = plan.splits;
+    p.tiles_m = ceil_div(p.M, bnc); p.tiles_n = ceil_div(p.N, plan.pair ? 2 * BM_ROWS : BM_ROWS); p.tiles = p.tiles_m * p.tiles_n;
+    p.stage_bytes = BmCfg<KIND>::PARTS * (BM_ROWS * 128u + (uint32_t)(plan.pair ? plan.BN / 2 : plan.BN) * 128u);
+    p.stages = std::min<int>(BM_MAX_STAGES, BM_RING / p.stage_bytes);
+    if (p.splits > 1 && !(p.part = sc.scratch<uint32_t>((size_t)p.tiles * p.splits * BM_ROWS * plan.BN))) return false;
+    return p.status != nullptr;
+}
+
+static bool bm_ready()
+{
+    if (tc_encode_tiled_fn()) return true;
+    set_error(TL_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    return false;
+}
+static bool bm_no_map()
+{
+    set_error(TL_ERR_CUDA, "cuTensorMapEncodeTiled refused an operand");
+    return false;
+}
+template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> &f)
+{
+    constexpr int KIND = sizeof(T) == 2 ? MM_F16 : MM_TF32, BK = BmCfg<KIND>::BK;
+    constexpr long long EB = 16 / (long long)sizeof(T);
+    if (!bm_ready()) return false;
+    const int nb = EPI == FFN_GATE ? 2 : f.terms, Kp = (int)(((long long)f.K + EB - 1) / EB * EB);
+    struct Op { const T *at; long long os, ps; int mn; };
+    PackOps<T> pack[2];                                                              // a launch packs two operands at most
+    int blocks[2] = {0, 0}, packs = 0;
+    pack[0].count = pack[1].count = 0;
+    // one layout for all operands of a side: they share strides, and all are read in place or none
+    auto side = [&](const T *const *src, int count, long long rs, long long cs, int rows, Op *o) -> bool {
+        int where = tm_in_place<T>(src[0], rs, cs, 0, rows, f.K, 1);
+        if (count > 1 && tm_in_place<T>(src[1], rs, cs, 0, rows, f.K, 1) != where) where = 0;
+        for (int i = 0; i < count; i++) {
+            if (where) { o[i] = {src[i], where == 1 ? rs : cs, 0, where - 1}; continue; }
+            const size_t size = ((size_t)rows * Kp + 63) & ~(size_t)63;
+            T *hi = sc.scratch<T>(BmCfg<KIND>::PARTS * size);
+            if (!hi) return false;
+            PackOps<T> &q = pack[packs / 2];
+            int &nb_ = blocks[packs / 2];
+            packs++;
+            const bool straight = cs == 1;
+            PackOp<T> &op = q.op[q.count++];
+            op = {src[i], hi, sizeof(T) == 4 ? hi + size : nullptr, rs, cs, 0, rows, f.K, Kp, ceil_div(Kp, straight ? 64 : 32), ceil_div(rows, straight ? 32 : 64), nb_, straight,
+                  (straight ? rs : rs == 1 ? cs : 1) % EB == 0 && ((uintptr_t)src[i] & 15) == 0};
+            nb_ += op.nk * op.nr;
+            o[i] = {hi, Kp, (long long)size, 0};
+        }
+        return true;
+    };
+    Op a[2], b[2];
+    if (!side(f.A, f.terms, f.a_rs, f.a_cs, f.N, a) || !side(f.B, nb, f.b_cs, f.b_rs, f.M, b)) return false;
+    BmParams<T> p = {};
+    p.C = f.C; p.g = f.g; p.u = f.u; p.dg = f.dg; p.du = f.du; p.N = f.N; p.M = f.M;
+    p.kps = ceil_div(f.K, BK); p.ksteps = p.kps * f.terms;
+    p.a_mn = a[0].mn; p.b_mn = b[0].mn;
+    auto odd = [](const void *q) { return ((uintptr_t)q & 15) != 0; };
+    p.vec = f.M % EB == 0 && !odd(f.C) && !odd(f.g) && !odd(f.u) && !odd(f.dg) && !odd(f.du);
+    const BmPlan plan = bm_plan(KIND, EPI, f.N, f.M, p.ksteps);
+    if (!bm_setup<KIND, T, EPI>(sc, plan, p)) return false;
+    const CUtensorMapDataType type = sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    auto map_of = [&](CUtensorMap *m, const Op &o, int rows, int box_rows) -> bool {
+        return o.mn ? bm_map(m, type, (int)sizeof(T), o.at, rows, f.K, 1, o.os, 0, 64, 64) : bm_map(m, type, sizeof(T), o.at, f.K, rows, BmCfg<KIND>::PARTS, o.os, o.ps, BK, box_rows);
+    };
+    BmMaps maps;
+    const int b_rows = EPI == FFN_GATE ? plan.BN / 2 : plan.pair ? plan.BN / 2 : plan.BN;
+    for (int i = 0; i < 2; i++) {
+        if (!map_of(&maps.a[i], a[std::min(i, f.terms - 1)], f.N, BM_ROWS) || !map_of(&maps.b[i], b[std::min(i, nb - 1)], f.M, b_rows)) return bm_no_map();
+    }
+    for (int i = 0; i < 2; i++) if (pack[i].count) TL_LAUNCH((pack_kmajor_kernel<T>), blocks[i], 256, 0, pack[i]);
+    bm_dispatch<KIND, T, EPI>(plan, maps, p);
+    return true;
+}
+#define INST(T)                                                             \
+    template bool block_mm<T, FFN_PLAIN>(Scope &, const FfnProduct<T> &);   \
+    template bool block_mm<T, FFN_GATE>(Scope &, const FfnProduct<T> &);    \
+    template bool block_mm<T, FFN_GATE_BW>(Scope &, const FfnProduct<T> &);
+INST(float)
+INST(__half)
+
+// rows of `size` bytes that do not lie on 16-byte boundaries -> rows of `padded` bytes (behind the end: never read); a thread per 16 bytes
+__global__ void __launch_bounds__(256) pack_rows_int8_kernel(const signed char *__restrict__ src, uint4 *__restrict__ dst, int rows, int size, int quads)
+{
+    pdl_wait();
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= (long long)rows * quads) return;
+    const int r = (int)(e / quads), k = (int)(e - (long long)r * quads) * 16;
+    const signed char *s = src + (size_t)r * size + k;
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        w[q] = 0;
+#pragma unroll
+        for (int b = 0; b < 4; b++) if (k + 4 * q + b < size) w[q] |= (uint32_t)(unsigned char)s[4 * q + b] << (8 * b);
+    }
+    dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <class T> void linear_int8(Scope &sc, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out)
+{
+    if (!bm_ready()) return;
+    const int quads = ceil_div(in, 16);
+    const signed char *at[2] = {x, w};
+    signed char *copy[2] = {nullptr, nullptr};
+    const int count[2] = {rows, out};
+    for (int i = 0; i < 2; i++)
+        if (in % 16 || ((uintptr_t)at[i] & 15)) {
+            if (!(copy[i] = sc.scratch<signed char>((size_t)count[i] * quads * 16))) return;
+        }
+    BmParams<T> p = {};
+    p.C = y; p.bias = bias; p.xs = xs; p.ws = ws; p.N = rows; p.M = out;
+    p.kps = p.ksteps = ceil_div(in, BmCfg<MM_I8>::BK);
+    p.vec = out % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)y & 15) == 0;
+    const BmPlan plan = bm_plan(MM_I8, FFN_INT8, rows, out, p.ksteps);
+    if (!bm_setup<MM_I8, T, FFN_INT8>(sc, plan, p)) return;
+    BmMaps maps;
+    for (int i = 0; i < 2; i++)
+        if (!bm_map(i ? &maps.b[0] : &maps.a[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, copy[i] ? copy[i] : at[i], in, count[i], 1, copy[i] ? (long long)quads * 16 : in, 0, BmCfg<MM_I8>::BK,
+                    i ? (plan.pair ? plan.BN / 2 : plan.BN) : BM_ROWS)) { bm_no_map(); return; }
+    maps.a[1] = maps.a[0]; maps.b[1] = maps.b[0];
+    for (int i = 0; i < 2; i++)
+        if (copy[i]) TL_LAUNCH(pack_rows_int8_kernel, ceil_div((long long)count[i] * quads, 256), 256, 0, at[i], (uint4 *)copy[i], count[i], in, quads);
+    bm_dispatch<MM_I8, T, FFN_INT8>(plan, maps, p);
+}
+template void linear_int8<float>(Scope &, const signed char *, const float *, const signed char *, const float *, const float *, float *, int, int, int);
+template void linear_int8<__half>(Scope &, const signed char *, const float *, const signed char *, const float *, const __half *, __half *, int, int, int);
+
+} // namespace tl
