@@ -1,0 +1,274 @@
+// The forward products of the feed-forward block and the 8-bit linear layer for few tokens (a generation loop's): bound by the weights' bytes, which are
+// read once, straight into the registers that the matrix instruction takes them from.
+//   A CTA has 16 rows of the weights (32 where there are many tokens; 16 of each matrix for the gate) and all tokens; its eight warps share K in pieces of 64 bytes.  The
+//   order of K inside a piece does not matter to a sum as long as both operands keep it: a thread loads 16 neighbouring bytes of its two weight rows
+//   and of its token, and they serve as the fragments of two mma.sync (m16n8k16 fp16, m16n8k32 in 8 bits): no shared memory, no shuffles.
+//   The warps' sums meet in shared memory, in order.
+// Single precision: the same on FFMA, a warp's lanes along K, four rows at a time by up to eight tokens.
+#include "tl_gate.cuh"
+#include "tl_reduce.cuh"
+
+namespace tl {
+
+enum { FEW_F16 = 0, FEW_I8 = 1 };
+static constexpr int FEW_WARPS = 8;
+template <bool I8> struct FewType { typedef __half E; typedef float S; };
+template <> struct FewType<true> { typedef signed char E; typedef int S; };
+
+template <class T> struct FewParams {
+    const void *x, *w[2];
+    T *C, *g, *u;
+    const T *bias; const float *xs, *ws;
+    int rows, M, K;                     // tokens, weight rows, elements of K
+    long long x_stride, c_stride;       // elements
+};
+
+// 16 neighbouring bytes of a row of K elements from element k on (zeros behind the end), from addresses that are multiples of ALIGN bytes
+template <class E, int ALIGN> __device__ __forceinline__ uint4 few_load(const E *row, int k, int K)
+{
+    constexpr int N = 16 / (int)sizeof(E);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if constexpr (ALIGN == 16) { if (k < K) v = *reinterpret_cast<const uint4 *>(row + k); }
+    else if constexpr (ALIGN == 4) {
+        if (k < K) v.x = *reinterpret_cast<const uint32_t *>(row + k);
+        if (k + N / 4 < K) v.y = *reinterpret_cast<const uint32_t *>(row + k + N / 4);
+        if (k + N / 2 < K) v.z = *reinterpret_cast<const uint32_t *>(row + k + N / 2);
+        if (k + 3 * N / 4 < K) v.w = *reinterpret_cast<const uint32_t *>(row + k + 3 * N / 4);
+    } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            uint32_t e = 0;
+            if (k + i < K) { if constexpr (sizeof(E) == 2) e = *reinterpret_cast<const unsigned short *>(row + k + i); else e = *reinterpret_cast<const unsigned char *>(row + k + i); }
+            w[i * 4 / N] |= e << (i % (N / 4) * 8 * (int)sizeof(E));
+        }
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return v;
+}
+// Loads that are issued where they stand, all of a turn's in front of its first product: the weights past L1 (nobody reads them again), the tokens through it.
+__device__ __forceinline__ uint4 few_stream(const void *p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 few_keep(const void *p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void few_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// a result: v (and w, the second matrix') of token n and weight row m
+template <class T, int EPI, class S> __device__ __forceinline__ void few_result(const FewParams<T> &p, int n, int m, S v, S w)
+{
+    const long long at = n * p.c_stride + m;
+    if constexpr (EPI == FFN_GATE) {
+        if (p.g) { st(p.g + (long long)n * p.M + m, v); st(p.u + (long long)n * p.M + m, w); }
+        st(p.C + at, gate_fw<sizeof(T) == 2>(v, w));
+    } else if constexpr (EPI == FFN_INT8) st(p.C + at, (float)v * p.xs[n] * p.ws[m] + ld0(p.bias != nullptr, p.bias + m));
+    else st(p.C + at, v);
+}
+
+// NT: groups of eight tokens; MT: groups of 16 weight rows
+template <int KIND, class T, int EPI, int NT, int MT, int ALIGN>
+__global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_kernel(const __grid_constant__ FewParams<T> p)
+{
+    pdl_wait();
+    typedef typename FewType<KIND == FEW_I8>::E E;
+    typedef typename FewType<KIND == FEW_I8>::S S;
+    constexpr int MATS = EPI == FFN_GATE ? 2 : 1, N = 16 / (int)sizeof(E), PIECE = 4 * N;
+    constexpr int U = MATS * MT == 1 ? 4 : 2;            // pieces in flight: 128 bytes of weights per thread
+    __shared__ S red[FEW_WARPS][MATS * MT * NT * 4][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, m0 = blockIdx.x * 16 * MT;
+    const E *x = reinterpret_cast<const E *>(p.x);
+    S acc[MATS][MT][NT][4];
+#pragma unroll
+    for (int a = 0; a < MATS * MT * NT * 4; a++) (&acc[0][0][0][0])[a] = 0;
+    // rows behind the last are the last once more (their results are not written): no load has a condition
+    const E *wp[MATS][MT][2], *xp[NT];
+#pragma unroll
+    for (int b = 0; b < MATS; b++)
+#pragma unroll
+        for (int a = 0; a < MT; a++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) wp[b][a][h] = reinterpret_cast<const E *>(p.w[b]) + (long long)min(m0 + 16 * a + g + 8 * h, p.M - 1) * p.K;
+#pragma unroll
+    for (int n = 0; n < NT; n++) xp[n] = x + min(8 * n + g, p.rows - 1) * p.x_stride;
+    auto multiply = [&](const uint4 (&wv)[MATS][MT][2], const uint4 (&xv)[NT]) {
+#pragma unroll
+        for (int b = 0; b < MATS; b++)
+#pragma unroll
+            for (int a = 0; a < MT; a++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const uint4 lo = wv[b][a][0], hi = wv[b][a][1], y = xv[n];
+                    few_mma(acc[b][a][n], lo.x, hi.x, lo.y, hi.y, y.x, y.y);
+                    few_mma(acc[b][a][n], lo.z, hi.z, lo.w, hi.w, y.z, y.w);
+                }
+    };
+    int k0 = 0;
+    if constexpr (ALIGN == 16) {
+        for (; k0 + FEW_WARPS * PIECE * U <= p.K; k0 += FEW_WARPS * PIECE * U) {
+            uint4 wv[U][MATS][MT][2], xv[U][NT];
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const int k = k0 + (i * FEW_WARPS + warp) * PIECE + t * N;
+#pragma unroll
+                for (int b = 0; b < MATS; b++)
+#pragma unroll
+                    for (int a = 0; a < MT; a++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) wv[i][b][a][h] = few_stream(wp[b][a][h] + k);
+            }
+#pragma unroll
+            for (int i = 0; i < U; i++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) xv[i][n] = few_keep(xp[n] + k0 + (i * FEW_WARPS + warp) * PIECE + t * N);
+#pragma unroll
+            for (int i = 0; i < U; i++) multiply(wv[i], xv[i]);
+        }
+    }
+    for (; k0 < p.K; k0 += FEW_WARPS * PIECE) {
+        uint4 wv[MATS][MT][2], xv[NT];
+        const int k = k0 + warp * PIECE + t * N;
+#pragma unroll
+        for (int b = 0; b < MATS; b++)
+#pragma unroll
+            for (int a = 0; a < MT; a++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) wv[b][a][h] = few_load<E, ALIGN>(wp[b][a][h], k, p.K);
+#pragma unroll
+        for (int n = 0; n < NT; n++) xv[n] = few_load<E, ALIGN>(xp[n], k, p.K);
+        multiply(wv, xv);
+    }
+#pragma unroll
+    for (int a = 0; a < MATS * MT * NT * 4; a++) red[warp][a][lane] = (&acc[0][0][0][0])[a];
+    __syncthreads();
+    // accumulator c of lane (g, t): weight row g + 8 (c / 2), token 2 t + c % 2
+    for (int e = threadIdx.x; e < MT * 16 * NT * 8; e += 32 * FEW_WARPS) {
+        const int m = e % (MT * 16), n = e / (MT * 16);
+        if (n >= p.rows || m0 + m >= p.M) continue;
+        const int a = m / 16, r = m % 16, src = (r % 8) * 4 + (n % 8) / 2, c = (r / 8) * 2 + n % 2;
+        S v = 0, w = 0;
+#pragma unroll
+        for (int k = 0; k < FEW_WARPS; k++) {
+            v += red[k][(a * NT + n / 8) * 4 + c][src];
+            if constexpr (MATS == 2) w += red[k][((MT + a) * NT + n / 8) * 4 + c][src];
+        }
+        few_result<T, EPI, S>(p, n, m0 + m, v, w);
+    }
+}
+
+// Single precision: R rows of each matrix per CTA, its warps share K, lanes along it; NT tokens (blockIdx.y: which).  V: elements per load.
+template <int EPI, int NT, int R, int V>
+__global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_fp32_kernel(const __grid_constant__ FewParams<float> p)
+{
+    pdl_wait();
+    constexpr int MATS = EPI == FFN_GATE ? 2 : 1;
+    __shared__ float red[FEW_WARPS][MATS * R * NT];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = blockIdx.x * R, n0 = blockIdx.y * NT;
+    const float *x = reinterpret_cast<const float *>(p.x);
+    float acc[MATS][R][NT];
+#pragma unroll
+    for (int a = 0; a < MATS * R * NT; a++) (&acc[0][0][0])[a] = 0.f;
+#pragma unroll 2
+    for (int k = threadIdx.x * V; k < p.K; k += 32 * FEW_WARPS * V) {
+        float wv[MATS][R][V], xv[NT][V];
+        auto load = [&](const float *row, bool live, float (&v)[V]) {
+            if constexpr (V == 4) {
+                const float4 q = live ? *reinterpret_cast<const float4 *>(row + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+            } else v[0] = live ? row[k] : 0.f;
+        };
+#pragma unroll
+        for (int b = 0; b < MATS; b++)
+#pragma unroll
+            for (int r = 0; r < R; r++) load(reinterpret_cast<const float *>(p.w[b]) + (long long)(m0 + r) * p.K, m0 + r < p.M, wv[b][r]);
+#pragma unroll
+        for (int n = 0; n < NT; n++) load(x + (n0 + n) * p.x_stride, n0 + n < p.rows, xv[n]);
+#pragma unroll
+        for (int b = 0; b < MATS; b++)
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) acc[b][r][n] = fmaf(wv[b][r][v], xv[n][v], acc[b][r][n]);
+    }
+#pragma unroll
+    for (int a = 0; a < MATS * R * NT; a++) {
+        const float s = warp_sum((&acc[0][0][0])[a]);
+        if (lane == 0) red[warp][a] = s;
+    }
+    __syncthreads();
+    const int e = threadIdx.x;
+    if (e >= R * NT) return;
+    const int r = e % R, n = e / R;
+    if (n0 + n >= p.rows || m0 + r >= p.M) return;
+    float v = 0.f, w = 0.f;
+#pragma unroll
+    for (int k = 0; k < FEW_WARPS; k++) {
+        v += red[k][r * NT + n];
+        if constexpr (MATS == 2) w += red[k][(R + r) * NT + n];
+    }
+    few_result<float, EPI, float>(p, n0 + n, m0 + r, v, w);
+}
+
+template <int KIND, class T, int EPI, int ALIGN> static void few_launch(const FewParams<T> &p)
+{
+    constexpr int WIDE = EPI == FFN_GATE ? 1 : 2;
+    const int nt = ceil_div(p.rows, 8);
+    if (nt == 1) TL_LAUNCH((few_rows_kernel<KIND, T, EPI, 1, 1, ALIGN>), ceil_div(p.M, 16), 32 * FEW_WARPS, 0, p);
+    else if (nt == 2) TL_LAUNCH((few_rows_kernel<KIND, T, EPI, 2, 1, ALIGN>), ceil_div(p.M, 16), 32 * FEW_WARPS, 0, p);
+    else if (nt == 3) TL_LAUNCH((few_rows_kernel<KIND, T, EPI, 3, WIDE, ALIGN>), ceil_div(p.M, 16 * WIDE), 32 * FEW_WARPS, 0, p);
+    else TL_LAUNCH((few_rows_kernel<KIND, T, EPI, 4, WIDE, ALIGN>), ceil_div(p.M, 16 * WIDE), 32 * FEW_WARPS, 0, p);
+}
+template <int KIND, class T, int EPI> static void few_aligned(const FewParams<T> &p, int esize)
+{
+    const uintptr_t at = (uintptr_t)p.x | (uintptr_t)p.w[0] | (uintptr_t)(EPI == FFN_GATE ? p.w[1] : nullptr) | (uintptr_t)((long long)p.K * esize) | (uintptr_t)(p.x_stride * esize);
+    if (at % 16 == 0) few_launch<KIND, T, EPI, 16>(p);
+    else if (at % 4 == 0) few_launch<KIND, T, EPI, 4>(p);
+    else few_launch<KIND, T, EPI, 1>(p);
+}
+template <int EPI> static void few_fp32(const FewParams<float> &p)
+{
+    constexpr int R = EPI == FFN_GATE ? 2 : 4;
+    const bool wide = (((uintptr_t)p.x | (uintptr_t)p.w[0] | (uintptr_t)(EPI == FFN_GATE ? p.w[1] : nullptr)) & 15) == 0 && p.K % 4 == 0 && p.x_stride % 4 == 0;
+#define TL_FEW32(NT, V) TL_LAUNCH((few_rows_fp32_kernel<EPI, NT, R, V>), dim3(ceil_div(p.M, R), ceil_div(p.rows, NT)), 32 * FEW_WARPS, 0, p)
+    if (wide) { if (p.rows == 1) TL_FEW32(1, 4); else if (p.rows <= 4) TL_FEW32(4, 4); else TL_FEW32(8, 4); }
+    else { if (p.rows == 1) TL_FEW32(1, 1); else if (p.rows <= 4) TL_FEW32(4, 1); else TL_FEW32(8, 1); }
+#undef TL_FEW32
+}
+
+template <class T, int EPI> void few_rows_mm(const FfnProduct<T> &f, long long c_stride)
+{
+    FewParams<T> p = {};
+    p.x = f.A[0]; p.w[0] = f.B[0]; p.w[1] = f.B[1]; p.C = f.C; p.g = f.g; p.u = f.u; p.rows = f.N; p.M = f.M; p.K = f.K; p.x_stride = f.a_rs; p.c_stride = c_stride;
+    if constexpr (sizeof(T) == 2) few_aligned<FEW_F16, T, EPI>(p, 2);
+    else few_fp32<EPI>(p);
+}
+template <class T> void few_rows_int8(const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out)
+{
+    FewParams<T> p = {};
+    p.x = x; p.w[0] = w; p.C = y; p.bias = bias; p.xs = xs; p.ws = ws; p.rows = rows; p.M = out; p.K = in; p.x_stride = in; p.c_stride = out;
+    few_aligned<FEW_I8, T, FFN_INT8>(p, 1);
+}
+#define INST(T)                                                                 \
+    template void few_rows_mm<T, FFN_PLAIN>(const FfnProduct<T> &, long long);  \
+    template void few_rows_mm<T, FFN_GATE>(const FfnProduct<T> &, long long);   \
+    template void few_rows_int8<T>(const signed char *, const float *, const signed char *, const float *, const T *, T *, int, int, int);
+INST(float)
+INST(__half)
+
+} // namespace tl
