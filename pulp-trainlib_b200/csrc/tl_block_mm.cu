@@ -19,7 +19,7 @@ namespace tl {
 
 enum { MM_F16 = 0, MM_TF32 = 1, MM_I8 = 2 };
 static constexpr int BM_ROWS = 128, BM_EPI = 8, BM_THREADS = 32 * (BM_EPI + 2), BM_MAX_STAGES = 8;
-static constexpr uint32_t BM_RING = 200 * 1024;
+static constexpr uint32_t BM_RING = 192 * 1024;
 static constexpr int BM_CHUNK = 4;                     // fp32: K steps of 32 between two drains of the accumulators
 
 template <int KIND> struct BmCfg { static constexpr int BK = KIND == MM_F16 ? 64 : KIND == MM_TF32 ? 32 : 128, PARTS = KIND == MM_TF32 ? 2 : 1; };
@@ -106,28 +106,129 @@ template <int W> __device__ __forceinline__ void bm_ld(const __half *p, float (&
         for (int j = 0; j < W; j++) v[j] = ld0(j < live, p + j);
     }
 }
-// v: the accumulators (gate), w: the second ones (up); row and col are inside the result
-template <class T, int EPI, int W> __device__ __forceinline__ void bm_results(const BmParams<T> &p, int row, int col, float (&v)[W], float (&w)[W])
+// ---------------------------------------------------------------- tiles of 32 rows x W columns between a warp's registers and memory
+// In registers a lane has a row (as tensor memory gives it), in memory neighbouring lanes should have neighbouring columns: the tile turns in 2 KB of shared
+// memory per warp, 16-byte chunks XOR-swizzled with the row so that neither side has bank conflicts.  A lane storing its own row's 16 bytes
+// touches 32 lines per instruction; so the gradient's epilogue (two tensors in, three out) took 50000 cycles per tile, three times its products.
+template <class T, int W> struct BmTile {
+    static constexpr int CHUNKS = W * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);        // of a row; elements of a chunk
+    static __device__ __forceinline__ int at(int row, int chunk) { return (row * CHUNKS + (chunk ^ (row / (8 / CHUNKS) & (CHUNKS - 1)))) * 16; }
+    static __device__ __forceinline__ uint4 pack(const float *v)
+    {
+        if constexpr (sizeof(T) == 2) return make_uint4(bm_half2(v[0], v[1]), bm_half2(v[2], v[3]), bm_half2(v[4], v[5]), bm_half2(v[6], v[7]));
+        else return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    // registers -> memory; base: the tensor's element (first row of the warp, first column of the tile); rows, cols: how many of them exist
+    static __device__ __forceinline__ void store(T *base, int M, int rows, int cols, bool vec, const float (&v)[W], unsigned char *stage, int lane)
+    {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++) *reinterpret_cast<uint4 *>(stage + at(lane, c)) = pack(v + c * E);
+        __syncwarp();
+        if (vec && cols >= W) {
+#pragma unroll
+            for (int i = 0; i < CHUNKS; i++) {
+                const int r = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
+                const uint4 x = *reinterpret_cast<const uint4 *>(stage + at(r, c));
+                if (r < rows) *reinterpret_cast<uint4 *>(base + (size_t)r * M + c * E) = x;
+            }
+        } else
+            for (int e = lane; e < 32 * W; e += 32) {
+                const int r = e / W, c = e % W;
+                if (r < rows && c < cols) base[(size_t)r * M + c] = *reinterpret_cast<const T *>(stage + at(r, c / E) + c % E * (int)sizeof(T));
+            }
+        __syncwarp();
+    }
+    // memory -> registers in two steps, so that the loads can be under way long before the tile is needed
+    static __device__ __forceinline__ void fetch(const T *base, int M, int rows, int cols, bool vec, uint4 (&q)[CHUNKS], int lane)
+    {
+        if (!vec || cols < W) return;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; i++) {
+            const int r = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
+            q[i] = make_uint4(0, 0, 0, 0);
+            if (r < rows) q[i] = *reinterpret_cast<const uint4 *>(base + (size_t)r * M + c * E);
+        }
+    }
+    static __device__ __forceinline__ void turn(const T *base, int M, int rows, int cols, bool vec, const uint4 (&q)[CHUNKS], float (&v)[W], unsigned char *stage, int lane)
+    {
+        if (vec && cols >= W) {
+#pragma unroll
+            for (int i = 0; i < CHUNKS; i++) *reinterpret_cast<uint4 *>(stage + at(i * (32 / CHUNKS) + lane / CHUNKS, lane % CHUNKS)) = q[i];
+        } else
+            for (int e = lane; e < 32 * W; e += 32) {
+                const int r = e / W, c = e % W;
+                if (r < rows && c < cols) *reinterpret_cast<T *>(stage + at(r, c / E) + c % E * (int)sizeof(T)) = base[(size_t)r * M + c];
+            }
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(stage + at(lane, c));
+            if constexpr (sizeof(T) == 2) {
+                bm_unpack(x.x, v[c * E], v[c * E + 1]); bm_unpack(x.y, v[c * E + 2], v[c * E + 3]); bm_unpack(x.z, v[c * E + 4], v[c * E + 5]); bm_unpack(x.w, v[c * E + 6], v[c * E + 7]);
+            } else { v[c * E] = __uint_as_float(x.x); v[c * E + 1] = __uint_as_float(x.y); v[c * E + 2] = __uint_as_float(x.z); v[c * E + 3] = __uint_as_float(x.w); }
+        }
+        __syncwarp();
+    }
+};
+// The results of W columns from col on of the 32 rows from row0 on.  v: the accumulators (gate), w: the second ones (up); gq, uq: G and U as BmTile::fetch left them.
+template <class T, int EPI, int W>
+__device__ __forceinline__ void bm_tile_results(const BmParams<T> &p, int row0, int col, float (&v)[W], float (&w)[W], const uint4 (&gq)[BmTile<T, W>::CHUNKS],
+                                                const uint4 (&uq)[BmTile<T, W>::CHUNKS], unsigned char *stage, int lane)
+{
+    typedef BmTile<T, W> Tile;
+    constexpr bool FAST = sizeof(T) == 2;
+    const size_t at = (size_t)row0 * p.M + col;
+    const int rows = p.N - row0, cols = p.M - col;
+    const bool vec = p.vec;
+    if constexpr (EPI == FFN_GATE) {
+        if (p.g) { Tile::store(p.g + at, p.M, rows, cols, vec, v, stage, lane); Tile::store(p.u + at, p.M, rows, cols, vec, w, stage, lane); }
+#pragma unroll
+        for (int j = 0; j < W; j++) v[j] = gate_fw<FAST>(v[j], w[j]);
+    } else if constexpr (EPI == FFN_GATE_BW) {
+        float g[W], u[W];
+        Tile::turn(p.g + at, p.M, rows, cols, vec, gq, g, stage, lane);
+        Tile::turn(p.u + at, p.M, rows, cols, vec, uq, u, stage, lane);
+#pragma unroll
+        for (int j = 0; j < W; j++) { const float dh = v[j]; gate_bw<FAST>(g[j], u[j], dh, v[j], g[j], u[j]); }
+        Tile::store(p.dg + at, p.M, rows, cols, vec, g, stage, lane);
+        Tile::store(p.du + at, p.M, rows, cols, vec, u, stage, lane);
+    } else if constexpr (EPI == FFN_INT8) {
+        const float xs = ld0(lane < rows, p.xs + row0 + lane);
+        const bool even = cols >= W && ((uintptr_t)p.ws & 15) == 0;
+        float s[W];
+        bm_ld<W>(p.ws + col, s, cols, even);
+#pragma unroll
+        for (int j = 0; j < W; j++) v[j] = v[j] * xs * s[j];
+        if (p.bias) {
+            bm_ld<W>(p.bias + col, s, cols, cols >= W && ((uintptr_t)p.bias & 15) == 0);
+#pragma unroll
+            for (int j = 0; j < W; j++) v[j] += s[j];
+        }
+    }
+    Tile::store(p.C + at, p.M, rows, cols, vec, v, stage, lane);
+}
+// The same for four columns of a row (from partial tiles)
+template <class T, int EPI> __device__ __forceinline__ void bm_results(const BmParams<T> &p, int row, int col, float (&v)[4], float (&w)[4])
 {
     constexpr bool FAST = sizeof(T) == 2;
     const size_t at = (size_t)row * p.M + col;
     const int live = p.M - col;
     if constexpr (EPI == FFN_GATE) {
-        if (p.g) { bm_st<W>(p.g + at, v, live, p.vec); bm_st<W>(p.u + at, w, live, p.vec); }
+        if (p.g) { bm_st<4>(p.g + at, v, live, p.vec); bm_st<4>(p.u + at, w, live, p.vec); }
 #pragma unroll
-        for (int j = 0; j < W; j++) v[j] = gate_fw<FAST>(v[j], w[j]);
+        for (int j = 0; j < 4; j++) v[j] = gate_fw<FAST>(v[j], w[j]);
     } else if constexpr (EPI == FFN_GATE_BW) {
-        float g[W], u[W];
-        bm_ld<W>(p.g + at, g, live, p.vec); bm_ld<W>(p.u + at, u, live, p.vec);
+        float g[4], u[4];
+        bm_ld<4>(p.g + at, g, live, p.vec); bm_ld<4>(p.u + at, u, live, p.vec);
 #pragma unroll
-        for (int j = 0; j < W; j++) { const float dh = v[j]; gate_bw<FAST>(g[j], u[j], dh, v[j], g[j], u[j]); }
-        bm_st<W>(p.dg + at, g, live, p.vec); bm_st<W>(p.du + at, u, live, p.vec);
+        for (int j = 0; j < 4; j++) { const float dh = v[j]; gate_bw<FAST>(g[j], u[j], dh, v[j], g[j], u[j]); }
+        bm_st<4>(p.dg + at, g, live, p.vec); bm_st<4>(p.du + at, u, live, p.vec);
     } else if constexpr (EPI == FFN_INT8) {
         const float xs = p.xs[row];
 #pragma unroll
-        for (int j = 0; j < W; j++) v[j] = v[j] * xs * ld0(j < live, p.ws + col + j) + ld0(p.bias && j < live, p.bias + col + j);
+        for (int j = 0; j < 4; j++) v[j] = v[j] * xs * ld0(j < live, p.ws + col + j) + ld0(p.bias && j < live, p.bias + col + j);
     }
-    bm_st<W>(p.C + at, v, live, p.vec);
+    bm_st<4>(p.C + at, v, live, p.vec);
 }
 
 // tile -> row block, column block: eight row blocks share a sweep over the columns
@@ -149,11 +250,13 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
     constexpr uint32_t A_BYTES = BM_ROWS * 128u, B_BYTES = BNL * 128u;
     constexpr int NBUF = KIND == MM_TF32 && BN > 64 ? 1 : 2;
     constexpr uint32_t BUF_COLS = 256;
+    constexpr int W = CW < 64 / (int)sizeof(T) ? CW : 64 / (int)sizeof(T);                // columns that a warp's epilogue takes at a time
     extern __shared__ unsigned char bsm_raw[];
     const uint32_t sbase = (smem_u32(bsm_raw) + 1023u) & ~1023u;                    // swizzle atoms want 1024-byte alignment
     __shared__ uint64_t full[BM_MAX_STAGES], empty[BM_MAX_STAGES], acc_full[2], acc_empty[2], last_bar;
     __shared__ uint32_t tmem_slot;
     __shared__ int failed_s;
+    __shared__ __align__(16) unsigned char stages_out[BM_EPI][2048];
     volatile int *failed = &failed_s;
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -284,27 +387,30 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
         const int quarter = warp & 3, half = warp >> 2;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const int row_in = quarter * 32 + lane;
+        unsigned char *stage = stages_out[warp];
+        typedef BmTile<T, W> Tile;
         int it = 0;
         bool ok = true;
         for (int tile = first; tile < p.tiles && ok; tile += step) {
             int rb, cb;
             bm_locate(p, tile, rb, cb);
-            const int row = rb * ROWS + row_of_tile + row_in, col0 = cb * BNC + half * CW;
+            const int row0 = rb * ROWS + row_of_tile + quarter * 32, col0 = cb * BNC + half * CW;
             constexpr int NS = KIND == MM_TF32 ? CW : 1, NS2 = KIND == MM_TF32 && EPI == FFN_GATE ? CW : 1;
             float sum[NS], sum2[NS2];
-            auto take = [&](uint32_t d, int c, float (&v)[16]) {                    // 16 accumulators of this lane's row
-                uint32_t a[16];
-                tmem_ld16(d + c, a);
+            const bool whole = PAIR || p.splits == 1;                               // results leave from here, not partial tiles
+            auto take = [&](uint32_t d, int c, float (&v)[W]) {                     // W accumulators of this lane's row
+                uint32_t a[W];
+                if constexpr (W == 32) tmem_ld32w(d + c, a); else tmem_ld16w(d + c, a);
                 if constexpr (KIND == MM_TF32) {
-                    uint32_t b[16], x[16];
-                    tmem_ld16(d + BN + c, b); tmem_ld16(d + 2 * BN + c, x);
+                    uint32_t b[W], x[W];
+                    if constexpr (W == 32) { tmem_ld32w(d + BN + c, b); tmem_ld32w(d + 2 * BN + c, x); } else { tmem_ld16w(d + BN + c, b); tmem_ld16w(d + 2 * BN + c, x); }
                     tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] = __uint_as_float(a[j]) + (__uint_as_float(b[j]) + __uint_as_float(x[j]));
+                    for (int j = 0; j < W; j++) v[j] = __uint_as_float(a[j]) + (__uint_as_float(b[j]) + __uint_as_float(x[j]));
                 } else {
                     tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] = KIND == MM_I8 && p.splits == 1 ? (float)(int)a[j] : __uint_as_float(a[j]);
+                    for (int j = 0; j < W; j++) v[j] = KIND == MM_I8 && whole ? (float)(int)a[j] : __uint_as_float(a[j]);
                 }
             };
             auto release = [&](int buf) {                                           // the accumulators are in registers: they may be overwritten
@@ -319,16 +425,30 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                 tc_fence_after();
                 return there;
             };
+            uint4 gq[Tile::CHUNKS], uq[Tile::CHUNKS], gn[Tile::CHUNKS], un[Tile::CHUNKS];       // G and U of this piece and the next
+            auto fetch = [&](int c) {
+                if constexpr (EPI == FFN_GATE_BW) {
+                    if (!whole || row0 >= p.N || c >= CW || col0 + c >= p.M) return;
+                    const size_t at = (size_t)row0 * p.M + col0 + c;
+                    Tile::fetch(p.g + at, p.M, p.N - row0, p.M - col0 - c, p.vec, gn, lane);
+                    Tile::fetch(p.u + at, p.M, p.N - row0, p.M - col0 - c, p.vec, un, lane);
+                }
+            };
             uint32_t *mine = p.part + ((size_t)(tile * p.splits + rank) * BM_ROWS + row_in) * BN;        // row of the partial tile (splits > 1)
-            auto leave = [&](int c, float (&v)[16], float (&w)[16]) {
-                if (!PAIR && p.splits > 1) {
+            auto leave = [&](int c, float (&v)[W], float (&w)[W]) {
+                if (!whole) {
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
+                    for (int j = 0; j < W; j += 4) {
                         *reinterpret_cast<float4 *>(mine + half * CW + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                         if constexpr (EPI == FFN_GATE) *reinterpret_cast<float4 *>(mine + BNC + half * CW + c + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
                     }
-                } else if (row < p.N && col0 + c < p.M) bm_results<T, EPI, 16>(p, row, col0 + c, v, w);
+                } else if (row0 < p.N && col0 + c < p.M) bm_tile_results<T, EPI, W>(p, row0, col0 + c, v, w, gq, uq, stage, lane);
             };
+            auto turn_over = [&]() {
+#pragma unroll
+                for (int i = 0; i < Tile::CHUNKS; i++) { gq[i] = gn[i]; uq[i] = un[i]; }
+            };
+            fetch(0);
             if constexpr (KIND == MM_TF32) {
 #pragma unroll
                 for (int j = 0; j < NS; j++) sum[j] = 0.f;
@@ -339,25 +459,27 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                     if (!arrived(buf, use)) { ok = false; break; }
                     const uint32_t d = tmem + lane_addr + buf * BUF_COLS;
 #pragma unroll
-                    for (int c = 0; c < CW; c += 16) {
-                        float v[16];
+                    for (int c = 0; c < CW; c += W) {
+                        float v[W];
                         take(d, half * CW + c, v);
 #pragma unroll
-                        for (int j = 0; j < 16; j++) sum[c + j] += v[j];
+                        for (int j = 0; j < W; j++) sum[c + j] += v[j];
                         if constexpr (EPI == FFN_GATE) {
                             take(d, BNC + half * CW + c, v);
 #pragma unroll
-                            for (int j = 0; j < 16; j++) sum2[c + j] += v[j];
+                            for (int j = 0; j < W; j++) sum2[c + j] += v[j];
                         }
                     }
                     release(buf);
                 }
                 if (!ok) break;
 #pragma unroll
-                for (int c = 0; c < CW; c += 16) {
-                    float v[16], w[16];
+                for (int c = 0; c < CW; c += W) {
+                    float v[W], w[W];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) { v[j] = sum[c + j]; w[j] = EPI == FFN_GATE ? sum2[EPI == FFN_GATE ? c + j : 0] : 0.f; }
+                    for (int j = 0; j < W; j++) { v[j] = sum[c + j]; w[j] = EPI == FFN_GATE ? sum2[EPI == FFN_GATE ? c + j : 0] : 0.f; }
+                    turn_over();
+                    fetch(c + W);
                     leave(c, v, w);
                 }
             } else {
@@ -366,11 +488,13 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                 if (!arrived(buf, use)) { ok = false; break; }
                 const uint32_t d = tmem + lane_addr + buf * BUF_COLS;
 #pragma unroll 1
-                for (int c = 0; c < CW; c += 16) {
-                    float v[16], w[16];
+                for (int c = 0; c < CW; c += W) {
+                    float v[W], w[W];
+                    turn_over();
+                    fetch(c + W);
                     take(d, half * CW + c, v);
                     if constexpr (EPI == FFN_GATE) take(d, BNC + half * CW + c, w);
-                    if (c + 16 >= CW) release(buf);
+                    if (c + W >= CW) release(buf);
                     leave(c, v, w);
                 }
             }
@@ -415,7 +539,7 @@ template <int KIND, class T, int EPI, int BN> __global__ void __launch_bounds__(
     float v[4], w[4];
     bm_add_parts<KIND, BN>(src, p.splits, v);
     if constexpr (EPI == FFN_GATE) bm_add_parts<KIND, BN>(src + BNC, p.splits, w);
-    bm_results<T, EPI, 4>(p, row, col, v, w);
+    bm_results<T, EPI>(p, row, col, v, w);
 }
 
 // ---------------------------------------------------------------- launch

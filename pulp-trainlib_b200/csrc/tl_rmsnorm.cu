@@ -6,8 +6,11 @@
 // from there.  Rows that no CTA's registers hold (above 32768 elements forward, 16384 backward) are read twice.
 #include "tl_kernels.h"
 #include "tl_reduce.cuh"
+#include "tl_tc.cuh"
 
 namespace tl {
+
+int *tc_status_word();          // tl_conv_tc.cu
 
 enum { NORM_PLAIN = 0, NORM_INT8 = 1, QUANT_ROWS = 2 };
 
@@ -18,15 +21,33 @@ __device__ __forceinline__ float2 quant_factor(float m)
     const float up = m < 0x1p-100f ? 0x1p100f : 1.f;
     return make_float2(up, m > 0.f ? __fdiv_rn(127.f, m * up) : 0.f);
 }
-// v / (m / 127) to the nearest whole number.  The quotient in 32 bits is off by three roundings, 127 * 3 * 2^-24 at most; beside the border of two steps
-// (one value in ten thousand, and every exact tie) 64 bits decide.
-__device__ __forceinline__ int quant(float v, float2 f, float m)
+// v / (m / 127) to the nearest whole number, V values at a time into bytes.  Adding 1.5 * 2^23 leaves the nearest whole number (ties to even) in the low bits.
+// The quotient in 32 bits is off by three roundings, 127 * 3 * 2^-24 at most: where one of the values lies that near the border of two steps (a few
+// in a hundred thousand, and every exact tie), and in rows that are not finite, 64 bits decide.
+__device__ __noinline__ int quant_exact(float v, float m)
 {
-    float t = v * f.x;
-    t *= f.y;
-    float n = rintf(t);
-    if (fabsf(fabsf(t - n) - 0.5f) < 3e-5f) n = (float)rint((double)v / ((double)m / 127.0));
-    return __float2int_rn(fminf(fmaxf(n == n ? n : 0.f, -127.f), 127.f));
+    const double n = rint((double)v / ((double)m / 127.0));
+    return m > 0.f && n == n ? (int)fmin(fmax(n, -127.0), 127.0) : 0;
+}
+template <int V> __device__ __forceinline__ void quant(const float (&v)[V], float2 f, float m, bool finite, signed char (&q)[V])
+{
+    float off = 0.f;
+    uint32_t u[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float t = v[i] * f.x * f.y, s = __fadd_rn(t, 12582912.f), d = fabsf(__fsub_rn(t, __fsub_rn(s, 12582912.f)));
+        off = fmaxf(off, d);
+        u[i] = __float_as_uint(s);
+    }
+    if (off > 0.5f - 3e-5f || !finite) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float t = v[i] * f.x * f.y;
+            if (!finite || fabsf(__fsub_rn(t, __fsub_rn(__uint_as_float(u[i]), 12582912.f))) > 0.5f - 3e-5f) u[i] = (uint32_t)quant_exact(v[i], m);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) q[i] = (signed char)(u[i] & 255u);
 }
 // a row's scale from r, its largest magnitude and a sum that is finite if all of it is
 __device__ __forceinline__ float quant_scale(float r, float m, float sum) { return sum - sum == 0.f ? r * __fdiv_rn(m, 127.f) : sum * 0.f; }
@@ -46,17 +67,275 @@ template <class T, int V> __device__ __forceinline__ Pack<T, V> zerov()
     return z;
 }
 
-// Two values over the G threads of a row (sum and sum, or sum and maximum), the same for all of them.  Every thread of the block takes part.
-template <int G, bool MAX> __device__ __forceinline__ float2 row_reduce(float a, float b, float2 *red)
+// Two values over a warp, a sum and a sum or maximum, in five exchanges: after the first one the lower half has the first value and the upper half the second.
+template <bool MAX> __device__ __forceinline__ float warp_two(float a, float b)
 {
-    a = warp_sum(a);
-    b = MAX ? warp_max(b) : warp_sum(b);
-    if constexpr (G == 32) return make_float2(a, b);
-    const int lane = threadIdx.x & 31, w0 = threadIdx.x / G * (G / 32);
-    if (lane == 0) red[threadIdx.x >> 5] = make_float2(a, b);
+    const bool low = (threadIdx.x & 16) == 0;
+    float v = low ? a : b;
+    const float u = __shfl_xor_sync(0xffffffffu, low ? b : a, 16);
+    v = MAX && !low ? fmaxf(v, u) : v + u;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        const float x = __shfl_xor_sync(0xffffffffu, v, o);
+        v = MAX && !low ? fmaxf(v, x) : v + x;
+    }
+    return v;
+}
+// The same over the G threads of a row, for all of them; red: [warps of the block].  SYNC: the barrier between the warps' results and their sum.
+template <int G, bool MAX, class SYNC> __device__ __forceinline__ float2 two_reduce(float a, float b, float2 *red, SYNC sync)
+{
+    const float v = warp_two<MAX>(a, b);
+    if constexpr (G == 32) { sync(); return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16)); }
+    if ((threadIdx.x & 15) == 0) reinterpret_cast<float *>(&red[threadIdx.x >> 5])[threadIdx.x >> 4 & 1] = v;
+    sync();
+    const float2 *of = red + threadIdx.x / G * (G / 32);
+    float2 t = of[0];
+#pragma unroll
+    for (int k = 1; k < G / 32; k++) { const float2 x = of[k]; t.x += x.x; t.y = MAX ? fmaxf(t.y, x.y) : t.y + x.y; }
+    return t;
+}
+template <int G, bool MAX> __device__ __forceinline__ float2 row_reduce(float a, float b, float2 *red)        // every thread of the block takes part
+{
+    return two_reduce<G, MAX>(a, b, red, [] { if (G > 32) __syncthreads(); });
+}
+
+// W results of a row: h (the unrounded sum) and the weights of V neighbouring columns
+template <class T, int MODE, int V>
+__device__ __forceinline__ void norm_leave(float (&h)[V], const Pack<T, V> &wv, float r, float2 f, float2 tot, T *sum, T *y, signed char *q, size_t at)
+{
+    if (MODE != QUANT_ROWS && sum) {
+        Pack<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++) o.e[i] = fromf<T>(h[i]);
+        stv<T, V>(sum + at, o);
+    }
+    if constexpr (MODE == NORM_PLAIN) {
+        Pack<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++) o.e[i] = fromf<T>(h[i] * r * tof(wv.e[i]));
+        stv<T, V>(y + at, o);
+    } else {
+        Pack<signed char, V> o;
+        if (MODE == NORM_INT8) {
+#pragma unroll
+            for (int i = 0; i < V; i++) h[i] *= tof(wv.e[i]);
+        }
+        quant<V>(h, f, tot.y, tot.x - tot.x == 0.f, o.e);
+        stv<signed char, V>(q + at, o);
+    }
+}
+// dw's partial sum of a block from its RG groups of rows, one behind the other
+template <class T, int G, int NV, int V, int RG, int TPB>
+__device__ __forceinline__ void block_columns(const float (&acc)[NV][V], float *out, float *cols, int size, int t, int mine)
+{
+    if constexpr (RG == 1) {
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < V; i++) { const int j = (k * G + t) * V + i; if (j < size) out[j] = acc[k][i]; }
+    } else {
+        for (int g = 0; g < RG; g++) {
+            __syncthreads();
+            if (mine != g) continue;
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int i = 0; i < V; i++) { const int j = (k * G + t) * V + i; if (j < size) cols[j] = g ? cols[j] + acc[k][i] : acc[k][i]; }
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < size; j += TPB) out[j] = cols[j];
+    }
+}
+
+// ---------------------------------------------------------------- rows through a ring in shared memory
+// Many rows: one CTA per SM whose groups of G threads walk rows of their own.  A group's rows arrive by bulk copies in a ring of stages (IN tensors' rows each),
+// some 200 KB under way per SM whatever the registers hold; a group waits for nobody but its own G threads.  A stage is fetched anew as soon as the
+// group's sums have met: by then all of it is in registers.
+static constexpr int RING_TPB = 512, RING_BYTES = 200 * 1024, RING_MOST = 8;
+template <int G> __device__ __forceinline__ void group_sync()
+{
+    if constexpr (G == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / G), "n"(G) : "memory");
+}
+template <int G, bool MAX> __device__ __forceinline__ float2 group_reduce(float a, float b, float2 *red) { return two_reduce<G, MAX>(a, b, red, [] { group_sync<G>(); }); }
+template <class T, int G, int IN> struct Ring {
+    const T *src[IN];
+    unsigned char *base;
+    uint64_t *full;
+    volatile int *failed;
+    int *status;
+    int stages, size, rows, row0, step, count;           // of this group: first row, rows between two of its rows, how many
+    int issued;                                          // (of the thread that fetches)
+    __device__ __forceinline__ T *stage(int s, int in) const { return reinterpret_cast<T *>(base) + ((size_t)s * IN + in) * size; }
+    __device__ __forceinline__ void issue(int i)
+    {
+        const int s = i % stages;
+        issued = i + 1;
+        const size_t at = (size_t)(row0 + (long long)i * step) * size;
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < IN; k++) n += src[k] != nullptr;
+        tc::mbar_arrive_expect_tx(&full[s], (uint32_t)(n * size * (int)sizeof(T)));
+#pragma unroll
+        for (int k = 0; k < IN; k++) if (src[k]) tc::bulk_load(stage(s, k), src[k] + at, (uint32_t)(size * sizeof(T)), &full[s]);
+    }
+    // Bounded: after about a second the CTA's flag is up, nothing is fetched any more and the other waits end at once (all threads keep walking, so that no
+    // barrier is short of one); the status word tells.
+    __device__ __forceinline__ void wait(int i)
+    {
+        uint64_t *bar = &full[i % stages];
+        const uint32_t parity = (uint32_t)(i / stages) & 1u;
+        for (uint32_t k = 0; k < 8000000u; k++) {
+            if (tc::mbar_try_wait(bar, parity)) return;
+            if ((k & 63u) == 63u && *failed) return;
+        }
+        *failed = 1;
+        atomicCAS(status, 0, 10);
+    }
+    __device__ __forceinline__ void start(int t) { if (t == 0) for (int i = 0; i < min(stages, count); i++) issue(i); }
+    __device__ __forceinline__ void refill(int i, int t) { if (t == 0 && i + stages < count && !*failed) issue(i + stages); }
+    // given up: what is under way lands before the shared memory is left
+    __device__ __forceinline__ void settle(int t)
+    {
+        if (t != 0 || !*failed) return;
+        for (int i = max(0, issued - stages); i < issued; i++)
+            for (int k = 0; k < 100000 && !tc::mbar_try_wait(&full[i % stages], (uint32_t)(i / stages) & 1u); k++) __nanosleep(100);
+    }
+};
+template <class T, int G, int IN> __device__ __forceinline__ Ring<T, G, IN> make_ring(unsigned char *mem, uint64_t (*full)[RING_MOST], int *failed, int *status, int stages, int size, int rows)
+{
+    constexpr int RG = RING_TPB / G;
+    const int mine = threadIdx.x / G;
+    Ring<T, G, IN> r;
+    r.base = mem + (size_t)mine * stages * IN * size * sizeof(T);
+    r.full = full[mine]; r.failed = failed; r.status = status;
+    r.stages = stages; r.size = size; r.rows = rows;
+    r.row0 = blockIdx.x * RG + mine; r.step = gridDim.x * RG;
+    r.count = r.row0 < rows ? (rows - 1 - r.row0) / r.step + 1 : 0;
+    r.issued = 0;
+    if (threadIdx.x < RG) for (int s = 0; s < stages; s++) tc::mbar_init(&full[threadIdx.x][s], 1);
+    if (threadIdx.x == 0) *failed = 0;
+    tc::fence_barrier_init();
     __syncthreads();
-    const float2 v = lane < G / 32 ? red[w0 + lane] : make_float2(0.f, 0.f);
-    return make_float2(warp_sum(v.x), MAX ? warp_max(v.y) : warp_sum(v.y));
+    return r;
+}
+
+template <class T, int MODE, int G, int NV, int V>
+__global__ void __launch_bounds__(RING_TPB) rmsnorm_fw_ring_kernel(const T *x, const T *res, const T *__restrict__ w, T *sum, T *y, signed char *__restrict__ q,
+                                                                   float *__restrict__ scale, int rows, int size, int stages, float eps, int *status)
+{
+    pdl_wait();
+    constexpr int IN = MODE == QUANT_ROWS ? 1 : 2;
+    extern __shared__ __align__(128) unsigned char ring_mem[];
+    __shared__ uint64_t full[RING_TPB / G][RING_MOST];
+    __shared__ float2 red[2][RING_TPB / 32];
+    __shared__ int failed;
+    Ring<T, G, IN> ring = make_ring<T, G, IN>(ring_mem, full, &failed, status, stages, size, rows);
+    ring.src[0] = x;
+    if constexpr (IN > 1) ring.src[1] = res;
+    const int t = threadIdx.x % G;
+    ring.start(t);
+    Pack<T, V> wv[NV];
+#pragma unroll
+    for (int k = 0; k < NV; k++) { const int j = (k * G + t) * V; wv[k] = MODE != QUANT_ROWS && j < size ? ldv<T, V>(w + j) : zerov<T, V>(); }
+    for (int i = 0; i < ring.count; i++) {
+        const int row = ring.row0 + i * ring.step;
+        const size_t at = (size_t)row * size;
+        ring.wait(i);
+        float h[NV][V], s = 0.f, m = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int j = (k * G + t) * V;
+            const bool in = j < size;
+            const Pack<T, V> a = in ? ldv<T, V>(ring.stage(i % stages, 0) + j) : zerov<T, V>(), b = IN > 1 && in && res ? ldv<T, V>(ring.stage(i % stages, IN - 1) + j) : zerov<T, V>();
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                h[k][e] = IN > 1 ? tof(a.e[e]) + tof(b.e[e]) : tof(a.e[e]);
+                s = MODE == QUANT_ROWS ? fmaf(h[k][e], 0.f, s) : fmaf(h[k][e], h[k][e], s);
+                if (MODE != NORM_PLAIN) m = fmaxf(m, fabsf(MODE == NORM_INT8 ? h[k][e] * tof(wv[k].e[e]) : h[k][e]));
+            }
+        }
+        const float2 tot = group_reduce<G, true>(s, m, red[i & 1]);
+        ring.refill(i, t);
+        const float r = MODE == QUANT_ROWS ? 1.f : 1.f / sqrtf(tot.x / (float)size + eps);
+        const float2 f = MODE == NORM_PLAIN ? make_float2(0.f, 0.f) : quant_factor(tot.y);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int j = (k * G + t) * V;
+            if (j < size) norm_leave<T, MODE, V>(h[k], wv[k], r, f, tot, sum, y, q, at + j);
+        }
+        if (MODE != NORM_PLAIN && t == 0) scale[row] = quant_scale(r, tot.y, tot.x);
+    }
+    ring.settle(t);
+}
+// backward: as rmsnorm_bw_kernel, below
+template <class T, int G, int NV, int V>
+__global__ void __launch_bounds__(RING_TPB) rmsnorm_bw_ring_kernel(const T *h, const T *__restrict__ w, const T *dy, const T *dsum, T *dx, float *__restrict__ part,
+                                                                   int rows, int size, int stages, float eps, int *status)
+{
+    pdl_wait();
+    constexpr int RG = RING_TPB / G;
+    extern __shared__ __align__(128) unsigned char ring_mem[];
+    __shared__ uint64_t full[RG][RING_MOST];
+    __shared__ float2 red[2][RING_TPB / 32];
+    __shared__ int failed;
+    Ring<T, G, 3> ring = make_ring<T, G, 3>(ring_mem, full, &failed, status, stages, size, rows);
+    ring.src[0] = h; ring.src[1] = dy; ring.src[2] = dx ? dsum : nullptr;
+    const int t = threadIdx.x % G, mine = threadIdx.x / G;
+    ring.start(t);
+    Pack<T, V> wv[NV];
+    float acc[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int j = (k * G + t) * V;
+        wv[k] = j < size ? ldv<T, V>(w + j) : zerov<T, V>();
+#pragma unroll
+        for (int e = 0; e < V; e++) acc[k][e] = 0.f;
+    }
+    for (int i = 0; i < ring.count; i++) {
+        const size_t at = (size_t)(ring.row0 + i * ring.step) * size;
+        ring.wait(i);
+        Pack<T, V> hv[NV], gv[NV], dv[NV];
+        float s = 0.f, c = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int j = (k * G + t) * V;
+            hv[k] = gv[k] = dv[k] = zerov<T, V>();
+            if (j < size) {
+                hv[k] = ldv<T, V>(ring.stage(i % stages, 0) + j); gv[k] = ldv<T, V>(ring.stage(i % stages, 1) + j);
+                if (ring.src[2]) dv[k] = ldv<T, V>(ring.stage(i % stages, 2) + j);
+            }
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float v = tof(hv[k].e[e]);
+                s = fmaf(v, v, s);
+                c = fmaf(v, tof(gv[k].e[e]) * tof(wv[k].e[e]), c);
+            }
+        }
+        const float2 tot = group_reduce<G, false>(s, c, red[i & 1]);
+        ring.refill(i, t);
+        const float r = 1.f / sqrtf(tot.x / (float)size + eps), cr = tot.y / (float)size * r * r;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int j = (k * G + t) * V;
+            Pack<T, V> o;
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float v = tof(hv[k].e[e]), g = tof(gv[k].e[e]);
+                acc[k][e] = fmaf(g * v, r, acc[k][e]);
+                o.e[e] = fromf<T>(tof(dv[k].e[e]) + r * (g * tof(wv[k].e[e]) - v * cr));
+            }
+            if (dx && j < size) stv<T, V>(dx + at + j, o);
+        }
+    }
+    ring.settle(t);
+    if (part) block_columns<T, G, NV, V, RG, RING_TPB>(acc, part + (size_t)blockIdx.x * size, reinterpret_cast<float *>(ring_mem), size, t, mine);
+}
+// stages per group, or 0: the rows are too long for two
+template <class T> static int ring_stages(int groups, int in, int size)
+{
+    const int n = RING_BYTES / (groups * in * size * (int)sizeof(T));
+    return n < 2 ? 0 : std::min(n, RING_MOST);
 }
 
 // ---------------------------------------------------------------- forward
@@ -96,24 +375,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) rmsnorm_fw_kernel(const T *
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int j = (k * G + t) * V;
-        if (j >= size) continue;
-        if (MODE != QUANT_ROWS && sum) {
-            Pack<T, V> o;
-#pragma unroll
-            for (int i = 0; i < V; i++) o.e[i] = fromf<T>(h[k][i]);
-            stv<T, V>(sum + at + j, o);
-        }
-        if constexpr (MODE == NORM_PLAIN) {
-            Pack<T, V> o;
-#pragma unroll
-            for (int i = 0; i < V; i++) o.e[i] = fromf<T>(h[k][i] * r * tof(wv[k].e[i]));
-            stv<T, V>(y + at + j, o);
-        } else {
-            Pack<signed char, V> o;
-#pragma unroll
-            for (int i = 0; i < V; i++) o.e[i] = (signed char)quant(MODE == NORM_INT8 ? h[k][i] * tof(wv[k].e[i]) : h[k][i], f, tot.y);
-            stv<signed char, V>(q + at + j, o);
-        }
+        if (j < size) norm_leave<T, MODE, V>(h[k], wv[k], r, f, tot, sum, y, q, at + j);
     }
     if (MODE != NORM_PLAIN && t == 0) scale[row] = quant_scale(r, tot.y, tot.x);
 }
@@ -139,7 +401,12 @@ __global__ void __launch_bounds__(1024) rmsnorm_fw_wide_kernel(const T *x, const
         const float h = ld(x + at + j) + (res ? ld(res + at + j) : 0.f);
         if (MODE != QUANT_ROWS && sum) st(sum + at + j, h);
         if (MODE == NORM_PLAIN) st(y + at + j, h * r * ld(w + j));
-        else q[at + j] = (signed char)quant(MODE == NORM_INT8 ? h * ld(w + j) : h, f, tot.y);
+        else {
+            const float v[1] = {MODE == NORM_INT8 ? h * ld(w + j) : h};
+            signed char o[1];
+            quant<1>(v, f, tot.y, tot.x - tot.x == 0.f, o);
+            q[at + j] = o[0];
+        }
     }
     if (MODE != NORM_PLAIN && threadIdx.x == 0) scale[blockIdx.x] = quant_scale(r, tot.y, tot.x);
 }
@@ -164,6 +431,27 @@ static void norm_forward(const T *x, const T *res, const T *w, T *sum, T *y, sig
         else if (packs <= 2048) TL_NORM(1024, 2, V);                                                  \
         else TL_NORM(1024, 4, V);                                                                     \
     } while (0)
+    if (wide && rows >= 4 * sm_count() && size <= RING_TPB * 32) {
+        int *status = tc_status_word();
+        constexpr int IN = MODE == QUANT_ROWS ? 1 : 2;
+#define TL_NORM_RING(G, NV)                                                                                                                                       \
+    do {                                                                                                                                                          \
+        const int stages = status ? ring_stages<T>(RING_TPB / G, IN, size) : 0;                                                                                   \
+        if (!stages) break;                                                                                                                                       \
+        static bool set = false;                                                                                                                                  \
+        if (!set) set = cudaFuncSetAttribute(rmsnorm_fw_ring_kernel<T, MODE, G, NV, V16>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES) == cudaSuccess; \
+        TL_LAUNCH((rmsnorm_fw_ring_kernel<T, MODE, G, NV, V16>), sm_count(), RING_TPB, RING_BYTES, x, res, w, sum, y, q, scale, rows, size, stages, eps, status);  \
+        return;                                                                                                                                                   \
+    } while (0)
+        constexpr int E = 32 / V16;
+        if (size <= 32 * 16) TL_NORM_RING(32, E / 2);
+        else if (size <= 32 * 32) TL_NORM_RING(32, E);
+        else if (size <= 64 * 32) TL_NORM_RING(64, E);
+        else if (size <= 128 * 32) TL_NORM_RING(128, E);
+        else if (size <= 256 * 32) TL_NORM_RING(256, E);
+        else TL_NORM_RING(512, E);
+#undef TL_NORM_RING
+    }
     if (packs > 4096) TL_LAUNCH((rmsnorm_fw_wide_kernel<T, MODE>), rows, 1024, 0, x, res, w, sum, y, q, scale, size, eps);
     else if (wide) TL_NORM_V(V16);
     else TL_NORM_V(1);
@@ -203,7 +491,7 @@ __global__ void __launch_bounds__(G < NB_TPB ? NB_TPB : G) rmsnorm_bw_kernel(con
 #pragma unroll
         for (int i = 0; i < V; i++) acc[k][i] = 0.f;
     auto weight = [&](int k) { const int j = (k * G + t) * V; return j < size ? ldv<T, V>(w + j) : zerov<T, V>(); };       // (from L1: registers go to the rows)
-    auto fetch = [&](int row) {
+    auto fetch = [&](long long row) {
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int j = (k * G + t) * V;
@@ -214,8 +502,8 @@ __global__ void __launch_bounds__(G < NB_TPB ? NB_TPB : G) rmsnorm_bw_kernel(con
     };
     int turn = 0;
     if (PRE) fetch(blockIdx.x * RG + mine);
-    for (int base = blockIdx.x * RG; base < rows; base += gridDim.x * RG, turn ^= 1) {
-        const int row = base + mine;
+    for (long long base = (long long)blockIdx.x * RG; base < rows; base += (long long)gridDim.x * RG, turn ^= 1) {
+        const long long row = base + mine;
         const size_t at = (size_t)row * size;
         Pack<T, V> dv[NV], hc[NV], gc[NV];
         auto residual = [&]() {
@@ -240,7 +528,7 @@ __global__ void __launch_bounds__(G < NB_TPB ? NB_TPB : G) rmsnorm_bw_kernel(con
                 c = fmaf(v, tof(gc[k].e[i]) * tof(wk.e[i]), c);
             }
         }
-        if (PRE) fetch(row + (int)gridDim.x * RG);       // under way while the row's sums meet (dx may be one of the inputs: of this row, which is in registers)
+        if (PRE) fetch(row + (long long)gridDim.x * RG);       // under way while the row's sums meet (dx may be one of the inputs: of this row, which is in registers)
         const float2 tot = row_reduce<G, false>(s, c, red[turn]);
         if (!PRE) residual();
         const float r = 1.f / sqrtf(tot.x / (float)size + eps), cr = tot.y / (float)size * r * r;
@@ -258,25 +546,7 @@ __global__ void __launch_bounds__(G < NB_TPB ? NB_TPB : G) rmsnorm_bw_kernel(con
             if (dx && row < rows && j < size) stv<T, V>(dx + at + j, o);
         }
     }
-    if (!part) return;
-    float *out = part + (size_t)blockIdx.x * size;
-    if constexpr (RG == 1) {
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int i = 0; i < V; i++) { const int j = (k * G + t) * V + i; if (j < size) out[j] = acc[k][i]; }
-    } else {
-        for (int g = 0; g < RG; g++) {
-            __syncthreads();
-            if (mine != g) continue;
-#pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int i = 0; i < V; i++) { const int j = (k * G + t) * V + i; if (j < size) cols[j] = g ? cols[j] + acc[k][i] : acc[k][i]; }
-        }
-        __syncthreads();
-        for (int j = threadIdx.x; j < size; j += TPB) out[j] = cols[j];
-    }
+    if (part) block_columns<T, G, NV, V, RG, TPB>(acc, part + (size_t)blockIdx.x * size, cols, size, t, mine);
 }
 // dw from the blocks' partial sums: 32 columns by 32 slices of the blocks, each slice in order, the slices in order
 template <class T> __global__ void __launch_bounds__(1024) rmsnorm_bw_sum_kernel(const float *__restrict__ part, T *__restrict__ dw, int size, int blocks)
@@ -356,6 +626,29 @@ template <class T> void rmsnorm_bw(Scope &sc, const T *h, const T *w, const T *d
         }
         if (dx) TL_LAUNCH((rmsnorm_bw_dx_kernel<T>), rows, 1024, 0, h, w, dy, dsum, dx, stats, size);
         return;
+    }
+    if (wide && size <= RING_TPB * 16) {
+        int *status = tc_status_word();
+#define TL_NORM_BW_RING(G, NV)                                                                                                                                    \
+    do {                                                                                                                                                          \
+        const int stages = status ? ring_stages<T>(RING_TPB / G, 3, size) : 0, blocks = std::min(ceil_div(rows, RING_TPB / G), sm_count());                       \
+        if (!stages) break;                                                                                                                                       \
+        float *part = dw ? sc.scratch<float>((size_t)blocks * size) : nullptr;                                                                                    \
+        if (dw && !part) return;                                                                                                                                  \
+        static bool set = false;                                                                                                                                  \
+        if (!set) set = cudaFuncSetAttribute(rmsnorm_bw_ring_kernel<T, G, NV, V16>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES) == cudaSuccess;      \
+        TL_LAUNCH((rmsnorm_bw_ring_kernel<T, G, NV, V16>), blocks, RING_TPB, RING_BYTES, h, w, dy, dsum, dx, part, rows, size, stages, eps, status);               \
+        if (dw) norm_columns<T>(part, dw, size, blocks);                                                                                                          \
+        return;                                                                                                                                                   \
+    } while (0)
+        constexpr int E = 16 / V16;
+        if (size <= 32 * 8) TL_NORM_BW_RING(32, (E + 1) / 2);
+        else if (size <= 32 * 16) TL_NORM_BW_RING(32, E);
+        else if (size <= 128 * 8) TL_NORM_BW_RING(128, (E + 1) / 2);
+        else if (size <= 128 * 16) TL_NORM_BW_RING(128, E);
+        else if (size <= 256 * 16) TL_NORM_BW_RING(256, E);
+        else TL_NORM_BW_RING(512, E);
+#undef TL_NORM_BW_RING
     }
 #define TL_NORM_BW(G, NV, V, PRE)                                                                                                                             \
     do {                                                                                                                                                      \
