@@ -52,6 +52,13 @@ template <int V> __device__ __forceinline__ void quant(const float (&v)[V], floa
 // a row's scale from r, its largest magnitude and a sum that is finite if all of it is
 __device__ __forceinline__ float quant_scale(float r, float m, float sum) { return sum - sum == 0.f ? r * __fdiv_rn(m, 127.f) : sum * 0.f; }
 
+// 1 / sqrt(v): the hardware's value (off by 2^-22.9) and one step of Newton's method; v = inf gives 0
+__device__ __forceinline__ float norm_factor(float v)
+{
+    const float r = rsqrtf(v);
+    return v < INFINITY ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
+}
+
 // ---------------------------------------------------------------- V neighbouring elements
 template <class T, int V> struct alignas(sizeof(T) * V) Pack { T e[V]; };
 template <class T, int V> __device__ __forceinline__ Pack<T, V> ldv(const T *p) { return *reinterpret_cast<const Pack<T, V> *>(p); }
@@ -65,6 +72,54 @@ template <class T, int V> __device__ __forceinline__ Pack<T, V> zerov()
 #pragma unroll
     for (int i = 0; i < V; i++) z.e[i] = fromf<T>(0.f);
     return z;
+}
+
+// Pairs of single-precision values: one instruction for two products or sums, rounded as two.  What bounds these kernels beside the bytes is the number of
+// instructions per element (31 of them, one by one and with every load under a condition of its own, held the half-precision backward pass at 4 TB/s).
+__device__ __forceinline__ uint64_t pair_bits(float2 v) { return *reinterpret_cast<const uint64_t *>(&v); }
+__device__ __forceinline__ float2 pair(uint64_t v) { return *reinterpret_cast<const float2 *>(&v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+    return pair(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return pair(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+    return pair(d);
+}
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+template <int V> __device__ __forceinline__ void unpack(const Pack<float, V> &p, float2 (&f)[V / 2])
+{
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) f[i] = make_float2(p.e[2 * i], p.e[2 * i + 1]);
+}
+template <int V> __device__ __forceinline__ void unpack(const Pack<__half, V> &p, float2 (&f)[V / 2])
+{
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) f[i] = __half22float2(*reinterpret_cast<const __half2 *>(&p.e[2 * i]));
+}
+template <int V> __device__ __forceinline__ Pack<float, V> repack(const float2 (&f)[V / 2], float *)
+{
+    Pack<float, V> p;
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) { p.e[2 * i] = f[i].x; p.e[2 * i + 1] = f[i].y; }
+    return p;
+}
+template <int V> __device__ __forceinline__ Pack<__half, V> repack(const float2 (&f)[V / 2], __half *)
+{
+    Pack<__half, V> p;
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) *reinterpret_cast<__half2 *>(&p.e[2 * i]) = __float22half2_rn(f[i]);
+    return p;
 }
 
 // Two values over a warp, a sum and a sum or maximum, in five exchanges: after the first one the lower half has the first value and the upper half the second.
@@ -220,12 +275,39 @@ template <class T, int G, int IN> __device__ __forceinline__ Ring<T, G, IN> make
     return r;
 }
 
+// the 8-bit form of V values, as quant(); SCALED: a row's magnitudes may be so small that 127 / m is not finite (half precision has none such)
+template <int V, bool SCALED> __device__ __forceinline__ Pack<signed char, V> quant_pairs(const float2 (&v)[V / 2], float2 f, float m, bool finite)
+{
+    uint32_t u[V];
+    float off = 0.f;
+    const float2 fx = twice(f.x), fy = twice(f.y), big = twice(12582912.f), less = twice(-12582912.f);
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) {
+        const float2 t = SCALED ? mul2(mul2(v[i], fx), fy) : mul2(v[i], fy), r = add2(t, big), n = add2(r, less), d = fma2(n, twice(-1.f), t);
+        off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+        u[2 * i] = __float_as_uint(r.x); u[2 * i + 1] = __float_as_uint(r.y);
+    }
+    if (off > 0.5f - 3e-5f || !finite) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float x = i & 1 ? v[i / 2].y : v[i / 2].x, t = x * f.x * f.y;
+            if (!finite || fabsf(__fsub_rn(t, __fsub_rn(__uint_as_float(u[i]), 12582912.f))) > 0.5f - 3e-5f) u[i] = (uint32_t)quant_exact(x, m);
+        }
+    }
+    Pack<signed char, V> q;
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<uint32_t *>(&q.e[i]) = __byte_perm(__byte_perm(u[i], u[i + 1], 0x0040), __byte_perm(u[i + 2], u[i + 3], 0x0040), 0x5410);
+    return q;
+}
+
 template <class T, int MODE, int G, int NV, int V>
 __global__ void __launch_bounds__(RING_TPB) rmsnorm_fw_ring_kernel(const T *x, const T *res, const T *__restrict__ w, T *sum, T *y, signed char *__restrict__ q,
                                                                    float *__restrict__ scale, int rows, int size, int stages, float eps, int *status)
 {
     pdl_wait();
-    constexpr int IN = MODE == QUANT_ROWS ? 1 : 2;
+    const float per = 1.f / (float)size;
+    constexpr int IN = MODE == QUANT_ROWS ? 1 : 2, P = V / 2;
+    constexpr bool HALVES = MODE == QUANT_ROWS && sizeof(T) == 2;
     extern __shared__ __align__(128) unsigned char ring_mem[];
     __shared__ uint64_t full[RING_TPB / G][RING_MOST];
     __shared__ float2 red[2][RING_TPB / 32];
@@ -238,31 +320,65 @@ __global__ void __launch_bounds__(RING_TPB) rmsnorm_fw_ring_kernel(const T *x, c
     Pack<T, V> wv[NV];
 #pragma unroll
     for (int k = 0; k < NV; k++) { const int j = (k * G + t) * V; wv[k] = MODE != QUANT_ROWS && j < size ? ldv<T, V>(w + j) : zerov<T, V>(); }
-    for (int i = 0; i < ring.count; i++) {
+    int s_at = 0;
+    for (int i = 0; i < ring.count; i++, s_at = s_at + 1 == stages ? 0 : s_at + 1) {
         const int row = ring.row0 + i * ring.step;
         const size_t at = (size_t)row * size;
         ring.wait(i);
-        float h[NV][V], s = 0.f, m = 0.f;
+        const T *in0 = ring.stage(s_at, 0), *in1 = ring.stage(s_at, IN - 1);
+        float2 h[NV][P], s2 = twice(0.f);
+        float m = 0.f;
+        Pack<T, V> raw[NV];
+        if constexpr (HALVES) {                              // largest magnitude as it lies, two halves at a time; NaN stays
+            __half2 m2 = __float2half2_rn(0.f);
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int j = (k * G + t) * V;
+                if (j >= size) continue;
+                raw[k] = ldv<T, V>(in0 + j);
+#pragma unroll
+                for (int e = 0; e < P; e++) m2 = __hmax2_nan(m2, __habs2(*reinterpret_cast<const __half2 *>(&raw[k].e[2 * e])));
+            }
+            m = __half2float(__hmax_nan(__low2half(m2), __high2half(m2)));
+            s2 = twice(m * 0.f);
+        } else
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int j = (k * G + t) * V;
-            const bool in = j < size;
-            const Pack<T, V> a = in ? ldv<T, V>(ring.stage(i % stages, 0) + j) : zerov<T, V>(), b = IN > 1 && in && res ? ldv<T, V>(ring.stage(i % stages, IN - 1) + j) : zerov<T, V>();
+            if (j >= size) continue;
+            unpack<V>(ldv<T, V>(in0 + j), h[k]);
+            if (IN > 1 && res) {
+                float2 b[P];
+                unpack<V>(ldv<T, V>(in1 + j), b);
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                h[k][e] = IN > 1 ? tof(a.e[e]) + tof(b.e[e]) : tof(a.e[e]);
-                s = MODE == QUANT_ROWS ? fmaf(h[k][e], 0.f, s) : fmaf(h[k][e], h[k][e], s);
-                if (MODE != NORM_PLAIN) m = fmaxf(m, fabsf(MODE == NORM_INT8 ? h[k][e] * tof(wv[k].e[e]) : h[k][e]));
+                for (int e = 0; e < P; e++) h[k][e] = add2(h[k][e], b[e]);
+            }
+            float2 ww[P];
+            if (MODE == NORM_INT8) unpack<V>(wv[k], ww);
+#pragma unroll
+            for (int e = 0; e < P; e++) {
+                s2 = fma2(h[k][e], MODE == QUANT_ROWS ? twice(0.f) : h[k][e], s2);       // (quantised alone, the sum tells only whether every value is finite)
+                if (MODE != NORM_PLAIN) { const float2 v = MODE == NORM_INT8 ? mul2(h[k][e], ww[e]) : h[k][e]; m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))); }
             }
         }
-        const float2 tot = group_reduce<G, true>(s, m, red[i & 1]);
+        const float2 tot = group_reduce<G, true>(s2.x + s2.y, m, red[i & 1]);
         ring.refill(i, t);
-        const float r = MODE == QUANT_ROWS ? 1.f : 1.f / sqrtf(tot.x / (float)size + eps);
+        const float r = MODE == QUANT_ROWS ? 1.f : norm_factor(fmaf(tot.x, per, eps));
         const float2 f = MODE == NORM_PLAIN ? make_float2(0.f, 0.f) : quant_factor(tot.y);
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int j = (k * G + t) * V;
-            if (j < size) norm_leave<T, MODE, V>(h[k], wv[k], r, f, tot, sum, y, q, at + j);
+            if (j >= size) continue;
+            if (MODE != QUANT_ROWS && sum) stv<T, V>(sum + at + j, repack<V>(h[k], (T *)nullptr));
+            if (MODE != QUANT_ROWS) {
+                float2 ww[P];
+                unpack<V>(wv[k], ww);
+#pragma unroll
+                for (int e = 0; e < P; e++) h[k][e] = mul2(MODE == NORM_PLAIN ? mul2(h[k][e], twice(r)) : h[k][e], ww[e]);
+            }
+            if constexpr (HALVES) unpack<V>(raw[k], h[k]);
+            if constexpr (MODE == NORM_PLAIN) stv<T, V>(y + at + j, repack<V>(h[k], (T *)nullptr));
+            else stv<signed char, V>(q + at + j, quant_pairs<V, sizeof(T) == 4 || MODE == NORM_INT8>(h[k], f, tot.y, tot.x - tot.x == 0.f));
         }
         if (MODE != NORM_PLAIN && t == 0) scale[row] = quant_scale(r, tot.y, tot.x);
     }
@@ -274,62 +390,73 @@ __global__ void __launch_bounds__(RING_TPB) rmsnorm_bw_ring_kernel(const T *h, c
                                                                    int rows, int size, int stages, float eps, int *status)
 {
     pdl_wait();
-    constexpr int RG = RING_TPB / G;
+    const float per = 1.f / (float)size;
+    constexpr int RG = RING_TPB / G, P = V / 2;
     extern __shared__ __align__(128) unsigned char ring_mem[];
     __shared__ uint64_t full[RG][RING_MOST];
     __shared__ float2 red[2][RING_TPB / 32];
     __shared__ int failed;
     Ring<T, G, 3> ring = make_ring<T, G, 3>(ring_mem, full, &failed, status, stages, size, rows);
     ring.src[0] = h; ring.src[1] = dy; ring.src[2] = dx ? dsum : nullptr;
+    const bool more = ring.src[2] != nullptr;
     const int t = threadIdx.x % G, mine = threadIdx.x / G;
     ring.start(t);
-    Pack<T, V> wv[NV];
-    float acc[NV][V];
+    float2 wv[NV][P], acc[NV][P];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int j = (k * G + t) * V;
-        wv[k] = j < size ? ldv<T, V>(w + j) : zerov<T, V>();
+        unpack<V>(j < size ? ldv<T, V>(w + j) : zerov<T, V>(), wv[k]);
 #pragma unroll
-        for (int e = 0; e < V; e++) acc[k][e] = 0.f;
+        for (int e = 0; e < P; e++) acc[k][e] = twice(0.f);
     }
-    for (int i = 0; i < ring.count; i++) {
+    int s_at = 0;
+    for (int i = 0; i < ring.count; i++, s_at = s_at + 1 == stages ? 0 : s_at + 1) {
         const size_t at = (size_t)(ring.row0 + i * ring.step) * size;
         ring.wait(i);
-        Pack<T, V> hv[NV], gv[NV], dv[NV];
-        float s = 0.f, c = 0.f;
+        const T *in_h = ring.stage(s_at, 0), *in_g = ring.stage(s_at, 1), *in_d = ring.stage(s_at, 2);
+        float2 hv[NV][P], gv[NV][P], s2 = twice(0.f), c2 = twice(0.f);
+        Pack<T, V> dv[NV];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int j = (k * G + t) * V;
-            hv[k] = gv[k] = dv[k] = zerov<T, V>();
-            if (j < size) {
-                hv[k] = ldv<T, V>(ring.stage(i % stages, 0) + j); gv[k] = ldv<T, V>(ring.stage(i % stages, 1) + j);
-                if (ring.src[2]) dv[k] = ldv<T, V>(ring.stage(i % stages, 2) + j);
-            }
+            if (j >= size) continue;
+            unpack<V>(ldv<T, V>(in_h + j), hv[k]);
+            unpack<V>(ldv<T, V>(in_g + j), gv[k]);
+            if (more) dv[k] = ldv<T, V>(in_d + j);
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float v = tof(hv[k].e[e]);
-                s = fmaf(v, v, s);
-                c = fmaf(v, tof(gv[k].e[e]) * tof(wv[k].e[e]), c);
+            for (int e = 0; e < P; e++) {
+                s2 = fma2(hv[k][e], hv[k][e], s2);
+                c2 = fma2(hv[k][e], mul2(gv[k][e], wv[k][e]), c2);
             }
         }
-        const float2 tot = group_reduce<G, false>(s, c, red[i & 1]);
+        const float2 tot = group_reduce<G, false>(s2.x + s2.y, c2.x + c2.y, red[i & 1]);
         ring.refill(i, t);
-        const float r = 1.f / sqrtf(tot.x / (float)size + eps), cr = tot.y / (float)size * r * r;
+        const float r = norm_factor(fmaf(tot.x, per, eps)), cr = tot.y * per * r * r;
+        const float2 rr = twice(r), less = twice(-cr);
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int j = (k * G + t) * V;
-            Pack<T, V> o;
+            if (j >= size) continue;
+            float2 d[P];
+            if (more) unpack<V>(dv[k], d);
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float v = tof(hv[k].e[e]), g = tof(gv[k].e[e]);
-                acc[k][e] = fmaf(g * v, r, acc[k][e]);
-                o.e[e] = fromf<T>(tof(dv[k].e[e]) + r * (g * tof(wv[k].e[e]) - v * cr));
+            for (int e = 0; e < P; e++) {
+                acc[k][e] = fma2(mul2(gv[k][e], hv[k][e]), rr, acc[k][e]);
+                const float2 v = fma2(hv[k][e], less, mul2(gv[k][e], wv[k][e]));
+                d[e] = more ? fma2(rr, v, d[e]) : mul2(rr, v);
             }
-            if (dx && j < size) stv<T, V>(dx + at + j, o);
+            if (dx) stv<T, V>(dx + at + j, repack<V>(d, (T *)nullptr));
         }
     }
     ring.settle(t);
-    if (part) block_columns<T, G, NV, V, RG, RING_TPB>(acc, part + (size_t)blockIdx.x * size, reinterpret_cast<float *>(ring_mem), size, t, mine);
+    if (part) {
+        float a[NV][V];
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int e = 0; e < P; e++) { a[k][2 * e] = acc[k][e].x; a[k][2 * e + 1] = acc[k][e].y; }
+        block_columns<T, G, NV, V, RG, RING_TPB>(a, part + (size_t)blockIdx.x * size, reinterpret_cast<float *>(ring_mem), size, t, mine);
+    }
 }
 // stages per group, or 0: the rows are too long for two
 template <class T> static int ring_stages(int groups, int in, int size)
@@ -345,6 +472,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) rmsnorm_fw_kernel(const T *
                                                                        float *__restrict__ scale, int rows, int size, float eps)
 {
     pdl_wait();
+    const float per = 1.f / (float)size;
     constexpr int TPB = G < 256 ? 256 : G;
     __shared__ float2 red[TPB / 32];
     const int row = blockIdx.x * (TPB / G) + threadIdx.x / G, t = threadIdx.x % G;
@@ -370,7 +498,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) rmsnorm_fw_kernel(const T *
         }
     const float2 tot = row_reduce<G, true>(s, m, red);
     if (row >= rows) return;
-    const float r = MODE == QUANT_ROWS ? 1.f : 1.f / sqrtf(tot.x / (float)size + eps);
+    const float r = MODE == QUANT_ROWS ? 1.f : norm_factor(fmaf(tot.x, per, eps));
     const float2 f = MODE == NORM_PLAIN ? make_float2(0.f, 0.f) : quant_factor(tot.y);
 #pragma unroll
     for (int k = 0; k < NV; k++) {
@@ -385,6 +513,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_fw_wide_kernel(const T *x, const
                                                                float *__restrict__ scale, int size, float eps)
 {
     pdl_wait();
+    const float per = 1.f / (float)size;
     __shared__ float2 red[32];
     const size_t at = (size_t)blockIdx.x * size;
     float s = 0.f, m = 0.f;
@@ -395,7 +524,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_fw_wide_kernel(const T *x, const
         if (MODE != NORM_PLAIN) m = fmaxf(m, fabsf(MODE == NORM_INT8 ? h * ld(w + j) : h));
     }
     const float2 tot = row_reduce<1024, true>(s, m, red);
-    const float r = MODE == QUANT_ROWS ? 1.f : 1.f / sqrtf(tot.x / (float)size + eps);
+    const float r = MODE == QUANT_ROWS ? 1.f : norm_factor(fmaf(tot.x, per, eps));
     const float2 f = quant_factor(tot.y);
     for (int j = threadIdx.x; j < size; j += 1024) {
         const float h = ld(x + at + j) + (res ? ld(res + at + j) : 0.f);
@@ -480,6 +609,7 @@ __global__ void __launch_bounds__(G < NB_TPB ? NB_TPB : G) rmsnorm_bw_kernel(con
                                                                             int rows, int size, float eps)
 {
     pdl_wait();
+    const float per = 1.f / (float)size;
     constexpr int TPB = G < NB_TPB ? NB_TPB : G, RG = TPB / G;
     __shared__ float2 red[2][TPB / 32];
     extern __shared__ float cols[];                      // [size], where RG > 1
@@ -531,7 +661,7 @@ __global__ void __launch_bounds__(G < NB_TPB ? NB_TPB : G) rmsnorm_bw_kernel(con
         if (PRE) fetch(row + (long long)gridDim.x * RG);       // under way while the row's sums meet (dx may be one of the inputs: of this row, which is in registers)
         const float2 tot = row_reduce<G, false>(s, c, red[turn]);
         if (!PRE) residual();
-        const float r = 1.f / sqrtf(tot.x / (float)size + eps), cr = tot.y / (float)size * r * r;
+        const float r = norm_factor(fmaf(tot.x, per, eps)), cr = tot.y * per * r * r;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int j = (k * G + t) * V;
@@ -570,6 +700,7 @@ template <class T>
 __global__ void __launch_bounds__(1024) rmsnorm_bw_stats_kernel(const T *__restrict__ h, const T *__restrict__ w, const T *__restrict__ dy, float2 *__restrict__ stats, int size, float eps)
 {
     pdl_wait();
+    const float per = 1.f / (float)size;
     __shared__ float2 red[32];
     const size_t at = (size_t)blockIdx.x * size;
     float s = 0.f, c = 0.f;
@@ -580,8 +711,8 @@ __global__ void __launch_bounds__(1024) rmsnorm_bw_stats_kernel(const T *__restr
         c = fmaf(v, ld(dy + at + j) * ld(w + j), c);
     }
     const float2 tot = row_reduce<1024, false>(s, c, red);
-    const float r = 1.f / sqrtf(tot.x / (float)size + eps);
-    if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(r, tot.y / (float)size * r * r);
+    const float r = norm_factor(fmaf(tot.x, per, eps));
+    if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(r, tot.y * per * r * r);
 }
 template <class T>
 __global__ void __launch_bounds__(128) rmsnorm_bw_cols_kernel(const T *__restrict__ h, const T *__restrict__ dy, const float2 *__restrict__ stats, float *__restrict__ part,
