@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(256) pack_rows_int8_kernel(const signed char *
 }
 template <class T> void linear_int8(Scope &sc, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out)
 {
-    if (rows <= FEW_ROWS) return few_rows_int8<T>(x, xs, w, ws, bias, y, rows, in, out);
+    if (rows <= FEW_ROWS) return few_rows_int8<T>(sc, x, xs, w, ws, bias, y, rows, in, out);
     if (!bm_ready()) return;
     const int quads = ceil_div(in, 16);
     const signed char *at[2] = {x, w};

@@ -1,17 +1,21 @@
 // The forward products of the feed-forward block and the 8-bit linear layer for few tokens (a generation loop's): bound by the weights' bytes, which are
 // read once, straight into the registers that the matrix instruction takes them from.
-//   A CTA has 16 rows of the weights (32 where there are many tokens; 16 of each matrix for the gate) and all tokens; its eight warps share K in pieces of 64 bytes.  The
-//   order of K inside a piece does not matter to a sum as long as both operands keep it: a thread loads 16 neighbouring bytes of its two weight rows
-//   and of its token, and they serve as the fragments of two mma.sync (m16n8k16 fp16, m16n8k32 in 8 bits): no shared memory, no shuffles.
-//   The warps' sums meet in shared memory, in order.
-// Single precision: the same on FFMA, a warp's lanes along K, four rows at a time by up to eight tokens.
+//   A CTA has 16 rows of the weights (16 of each matrix for the gate; 32 where there are many tokens and enough rows) and all tokens; its warps share K in
+//   pieces of 64 bytes.  The order of K inside a piece does not matter to a sum as long as both operands keep it: a thread loads 16 neighbouring bytes of
+//   its two weight rows and of its token, and they serve as the fragments of two mma.sync (m16n8k16 fp16, m16n8k32 in 8 bits): no shared memory, no
+//   shuffles.  The warps' sums meet in shared memory, in order.
+//   What counts is the number of loads under way: a thread issues all of a turn's, 256 bytes of weights, before it waits for the first.
+//   (Rings in shared memory with even shares of all bytes for persistent CTAs, by bulk copies of 1 KB or by cp.async, keep more under way, but lose more than
+//   that at the ends of the units: 8-bit 4096 -> 10240 for one token 16 us against 11, fp16 4096 x 10240 x 4096 57 us against 54.)
+//   Rows that do not start on 16 bytes come as the five words around the thread's bytes, shifted into place.
+// Single precision: the same on FFMA, a warp's lanes along K, a few rows at a time by up to eight tokens.
 #include "tl_gate.cuh"
 #include "tl_reduce.cuh"
 
 namespace tl {
 
 enum { FEW_F16 = 0, FEW_I8 = 1 };
-static constexpr int FEW_WARPS = 8;
+static constexpr int FEW_WARPS = 8;                  // of the single-precision kernel
 template <bool I8> struct FewType { typedef __half E; typedef float S; };
 template <> struct FewType<true> { typedef signed char E; typedef int S; };
 
@@ -23,18 +27,19 @@ template <class T> struct FewParams {
     long long x_stride, c_stride;       // elements
 };
 
-// 16 neighbouring bytes of a row of K elements from element k on (zeros behind the end), from addresses that are multiples of ALIGN bytes
+// 16 neighbouring bytes of a row of K elements from element k on, zeros behind the end.  ALIGN < 16: rows start anywhere.  Inside a row (four bytes in front of the
+// piece and behind it are the row's too) as whole words, at its ends element by element.
 template <class E, int ALIGN> __device__ __forceinline__ uint4 few_load(const E *row, int k, int K)
 {
-    constexpr int N = 16 / (int)sizeof(E);
+    constexpr int N = 16 / (int)sizeof(E), WORD = 4 / (int)sizeof(E);
     uint4 v = make_uint4(0, 0, 0, 0);
     if constexpr (ALIGN == 16) { if (k < K) v = *reinterpret_cast<const uint4 *>(row + k); }
-    else if constexpr (ALIGN == 4) {
-        if (k < K) v.x = *reinterpret_cast<const uint32_t *>(row + k);
-        if (k + N / 4 < K) v.y = *reinterpret_cast<const uint32_t *>(row + k + N / 4);
-        if (k + N / 2 < K) v.z = *reinterpret_cast<const uint32_t *>(row + k + N / 2);
-        if (k + 3 * N / 4 < K) v.w = *reinterpret_cast<const uint32_t *>(row + k + 3 * N / 4);
-    } else {
+    else if (k >= WORD && k + N + WORD <= K) {
+        const uintptr_t at = (uintptr_t)(row + k);
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3), sh = (uint32_t)(at & 3) * 8u;
+        const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = w[4];
+        v = make_uint4(__funnelshift_r(w0, w1, sh), __funnelshift_r(w1, w2, sh), __funnelshift_r(w2, w3, sh), __funnelshift_r(w3, w4, sh));
+    } else if (k < K) {
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -80,16 +85,17 @@ template <class T, int EPI, class S> __device__ __forceinline__ void few_result(
     else st(p.C + at, v);
 }
 
-// NT: groups of eight tokens; MT: groups of 16 weight rows
-template <int KIND, class T, int EPI, int NT, int MT, int ALIGN>
-__global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_kernel(const __grid_constant__ FewParams<T> p)
+// NT: groups of eight tokens; MT: groups of 16 weight rows; WARPS: that share K
+template <int KIND, class T, int EPI, int NT, int MT, int ALIGN, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const __grid_constant__ FewParams<T> p)
 {
     pdl_wait();
     typedef typename FewType<KIND == FEW_I8>::E E;
     typedef typename FewType<KIND == FEW_I8>::S S;
     constexpr int MATS = EPI == FFN_GATE ? 2 : 1, N = 16 / (int)sizeof(E), PIECE = 4 * N;
-    constexpr int U = MATS * MT == 1 ? 4 : 2;            // pieces in flight: 128 bytes of weights per thread
-    __shared__ S red[FEW_WARPS][MATS * MT * NT * 4][32];
+    // pieces of a turn: 256 bytes of weights per thread, 128 where the tokens take as many registers
+    constexpr int U = (NT > 1 ? 4 : 8) / (MATS * MT);
+    __shared__ S red[WARPS][MATS * MT * NT * 4][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, m0 = blockIdx.x * 16 * MT;
     const E *x = reinterpret_cast<const E *>(p.x);
     S acc[MATS][MT][NT][4];
@@ -119,11 +125,11 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_kernel(const __grid_c
     };
     int k0 = 0;
     if constexpr (ALIGN == 16) {
-        for (; k0 + FEW_WARPS * PIECE * U <= p.K; k0 += FEW_WARPS * PIECE * U) {
+        for (; k0 + WARPS * PIECE * U <= p.K; k0 += WARPS * PIECE * U) {
             uint4 wv[U][MATS][MT][2], xv[U][NT];
 #pragma unroll
             for (int i = 0; i < U; i++) {
-                const int k = k0 + (i * FEW_WARPS + warp) * PIECE + t * N;
+                const int k = k0 + (i * WARPS + warp) * PIECE + t * N;
 #pragma unroll
                 for (int b = 0; b < MATS; b++)
 #pragma unroll
@@ -134,35 +140,40 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < U; i++)
 #pragma unroll
-                for (int n = 0; n < NT; n++) xv[i][n] = few_keep(xp[n] + k0 + (i * FEW_WARPS + warp) * PIECE + t * N);
+                for (int n = 0; n < NT; n++) xv[i][n] = few_keep(xp[n] + k0 + (i * WARPS + warp) * PIECE + t * N);
 #pragma unroll
             for (int i = 0; i < U; i++) multiply(wv[i], xv[i]);
         }
     }
-    for (; k0 < p.K; k0 += FEW_WARPS * PIECE) {
-        uint4 wv[MATS][MT][2], xv[NT];
-        const int k = k0 + warp * PIECE + t * N;
+    constexpr int UT = ALIGN == 16 ? 1 : MT * MATS == 1 ? 4 : 2;
+    for (; k0 < p.K; k0 += WARPS * PIECE * UT) {
+        uint4 wv[UT][MATS][MT][2], xv[UT][NT];
 #pragma unroll
-        for (int b = 0; b < MATS; b++)
+        for (int i = 0; i < UT; i++) {
+            const int k = k0 + (i * WARPS + warp) * PIECE + t * N;
 #pragma unroll
-            for (int a = 0; a < MT; a++)
+            for (int b = 0; b < MATS; b++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) wv[b][a][h] = few_load<E, ALIGN>(wp[b][a][h], k, p.K);
+                for (int a = 0; a < MT; a++)
 #pragma unroll
-        for (int n = 0; n < NT; n++) xv[n] = few_load<E, ALIGN>(xp[n], k, p.K);
-        multiply(wv, xv);
+                    for (int h = 0; h < 2; h++) wv[i][b][a][h] = few_load<E, ALIGN>(wp[b][a][h], k, p.K);
+#pragma unroll
+            for (int n = 0; n < NT; n++) xv[i][n] = few_load<E, ALIGN>(xp[n], k, p.K);
+        }
+#pragma unroll
+        for (int i = 0; i < UT; i++) multiply(wv[i], xv[i]);
     }
 #pragma unroll
     for (int a = 0; a < MATS * MT * NT * 4; a++) red[warp][a][lane] = (&acc[0][0][0][0])[a];
     __syncthreads();
     // accumulator c of lane (g, t): weight row g + 8 (c / 2), token 2 t + c % 2
-    for (int e = threadIdx.x; e < MT * 16 * NT * 8; e += 32 * FEW_WARPS) {
+    for (int e = threadIdx.x; e < MT * 16 * NT * 8; e += 32 * WARPS) {
         const int m = e % (MT * 16), n = e / (MT * 16);
         if (n >= p.rows || m0 + m >= p.M) continue;
         const int a = m / 16, r = m % 16, src = (r % 8) * 4 + (n % 8) / 2, c = (r / 8) * 2 + n % 2;
         S v = 0, w = 0;
 #pragma unroll
-        for (int k = 0; k < FEW_WARPS; k++) {
+        for (int k = 0; k < WARPS; k++) {
             v += red[k][(a * NT + n / 8) * 4 + c][src];
             if constexpr (MATS == 2) w += red[k][((MT + a) * NT + n / 8) * 4 + c][src];
         }
@@ -225,21 +236,30 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_fp32_kernel(const __g
     few_result<float, EPI, float>(p, n0 + n, m0 + r, v, w);
 }
 
-template <int KIND, class T, int EPI, int ALIGN> static void few_launch(const FewParams<T> &p)
+template <int KIND, class T, int EPI, int NT, int MT, int ALIGN> static void few_launch(const FewParams<T> &p)
 {
-    constexpr int WIDE = EPI == FFN_GATE ? 1 : 2;
+    // fewer CTAs than SMs: twice the warps for each
+    const int ctas = ceil_div(p.M, 16 * MT);
+    constexpr int W = NT * MT * (EPI == FFN_GATE ? 2 : 1) <= 4 ? 16 : 8;           // (their sums fit the shared memory)
+    if (ctas <= sm_count() && W == 16) TL_LAUNCH((few_rows_kernel<KIND, T, EPI, NT, MT, ALIGN, W>), ctas, 32 * W, 0, p);
+    else TL_LAUNCH((few_rows_kernel<KIND, T, EPI, NT, MT, ALIGN, 8>), ctas, 256, 0, p);
+}
+template <int KIND, class T, int EPI, int ALIGN> static void few_tokens(const FewParams<T> &p)
+{
     const int nt = ceil_div(p.rows, 8);
-    if (nt == 1) TL_LAUNCH((few_rows_kernel<KIND, T, EPI, 1, 1, ALIGN>), ceil_div(p.M, 16), 32 * FEW_WARPS, 0, p);
-    else if (nt == 2) TL_LAUNCH((few_rows_kernel<KIND, T, EPI, 2, 1, ALIGN>), ceil_div(p.M, 16), 32 * FEW_WARPS, 0, p);
-    else if (nt == 3) TL_LAUNCH((few_rows_kernel<KIND, T, EPI, 3, WIDE, ALIGN>), ceil_div(p.M, 16 * WIDE), 32 * FEW_WARPS, 0, p);
-    else TL_LAUNCH((few_rows_kernel<KIND, T, EPI, 4, WIDE, ALIGN>), ceil_div(p.M, 16 * WIDE), 32 * FEW_WARPS, 0, p);
+    const bool wide = EPI != FFN_GATE && p.M > 32 * sm_count();
+    constexpr int WIDE = EPI != FFN_GATE ? 2 : 1;
+    if (nt == 1) few_launch<KIND, T, EPI, 1, 1, ALIGN>(p);
+    else if (nt == 2) few_launch<KIND, T, EPI, 2, 1, ALIGN>(p);
+    else if (nt == 3) { if (wide) few_launch<KIND, T, EPI, 3, WIDE, ALIGN>(p); else few_launch<KIND, T, EPI, 3, 1, ALIGN>(p); }
+    else if (wide) few_launch<KIND, T, EPI, 4, WIDE, ALIGN>(p);
+    else few_launch<KIND, T, EPI, 4, 1, ALIGN>(p);
 }
 template <int KIND, class T, int EPI> static void few_aligned(const FewParams<T> &p, int esize)
 {
     const uintptr_t at = (uintptr_t)p.x | (uintptr_t)p.w[0] | (uintptr_t)(EPI == FFN_GATE ? p.w[1] : nullptr) | (uintptr_t)((long long)p.K * esize) | (uintptr_t)(p.x_stride * esize);
-    if (at % 16 == 0) few_launch<KIND, T, EPI, 16>(p);
-    else if (at % 4 == 0) few_launch<KIND, T, EPI, 4>(p);
-    else few_launch<KIND, T, EPI, 1>(p);
+    if (at % 16 == 0) few_tokens<KIND, T, EPI, 16>(p);
+    else few_tokens<KIND, T, EPI, 1>(p);
 }
 template <int EPI> static void few_fp32(const FewParams<float> &p)
 {
@@ -251,23 +271,23 @@ template <int EPI> static void few_fp32(const FewParams<float> &p)
 #undef TL_FEW32
 }
 
-template <class T, int EPI> void few_rows_mm(const FfnProduct<T> &f, long long c_stride)
+template <class T, int EPI> void few_rows_mm(Scope &, const FfnProduct<T> &f, long long c_stride)
 {
     FewParams<T> p = {};
     p.x = f.A[0]; p.w[0] = f.B[0]; p.w[1] = f.B[1]; p.C = f.C; p.g = f.g; p.u = f.u; p.rows = f.N; p.M = f.M; p.K = f.K; p.x_stride = f.a_rs; p.c_stride = c_stride;
     if constexpr (sizeof(T) == 2) few_aligned<FEW_F16, T, EPI>(p, 2);
     else few_fp32<EPI>(p);
 }
-template <class T> void few_rows_int8(const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out)
+template <class T> void few_rows_int8(Scope &, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out)
 {
     FewParams<T> p = {};
     p.x = x; p.w[0] = w; p.C = y; p.bias = bias; p.xs = xs; p.ws = ws; p.rows = rows; p.M = out; p.K = in; p.x_stride = in; p.c_stride = out;
     few_aligned<FEW_I8, T, FFN_INT8>(p, 1);
 }
 #define INST(T)                                                                 \
-    template void few_rows_mm<T, FFN_PLAIN>(const FfnProduct<T> &, long long);  \
-    template void few_rows_mm<T, FFN_GATE>(const FfnProduct<T> &, long long);   \
-    template void few_rows_int8<T>(const signed char *, const float *, const signed char *, const float *, const T *, T *, int, int, int);
+    template void few_rows_mm<T, FFN_PLAIN>(Scope &, const FfnProduct<T> &, long long);  \
+    template void few_rows_mm<T, FFN_GATE>(Scope &, const FfnProduct<T> &, long long);   \
+    template void few_rows_int8<T>(Scope &, const signed char *, const float *, const signed char *, const float *, const T *, T *, int, int, int);
 INST(float)
 INST(__half)
 

@@ -34,7 +34,7 @@ template <class T> struct FfnProduct {
 template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> &p);
 // Few tokens (FEW_ROWS at most), weights with K contiguous (tl_few_rows.cu): FFN_PLAIN of one term and FFN_GATE.  c_stride: elements between the rows of C.
 static constexpr int FEW_ROWS = 32;
-template <class T, int EPI> void few_rows_mm(const FfnProduct<T> &p, long long c_stride);
-template <class T> void few_rows_int8(const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out);
+template <class T, int EPI> void few_rows_mm(Scope &sc, const FfnProduct<T> &p, long long c_stride);
+template <class T> void few_rows_int8(Scope &sc, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out);
 
 } // namespace tl

@@ -26,12 +26,12 @@ template <class T> void gated_ffn_fw(Scope &sc, const GatedFfn<T> &f)
     FfnProduct<T> p = {};
     p.A[0] = f.x; p.B[0] = f.wg; p.B[1] = f.wu; p.C = h; p.g = f.g; p.u = f.u; p.N = f.rows; p.M = f.hidden; p.K = f.in; p.terms = 1;
     p.a_rs = f.in; p.a_cs = 1; p.b_rs = 1; p.b_cs = f.in;
-    if (few) few_rows_mm<T, FFN_GATE>(p, pitch);
+    if (few) few_rows_mm<T, FFN_GATE>(sc, p, pitch);
     else if (!block_mm<T, FFN_GATE>(sc, p)) return;
     FfnProduct<T> d = {};
     d.A[0] = h; d.B[0] = f.wd; d.C = f.y; d.N = f.rows; d.M = f.out; d.K = f.hidden; d.terms = 1;
     d.a_rs = pitch; d.a_cs = 1; d.b_rs = 1; d.b_cs = f.hidden;
-    if (few) few_rows_mm<T, FFN_PLAIN>(d, f.out);
+    if (few) few_rows_mm<T, FFN_PLAIN>(sc, d, f.out);
     else block_mm<T, FFN_PLAIN>(sc, d);
 }
 template <class T> void gated_ffn_bw(Scope &sc, const GatedFfn<T> &f)
