@@ -24,15 +24,23 @@ static constexpr int BM_CHUNK = 4;                     // fp32: K steps of 32 be
 
 template <int KIND> struct BmCfg { static constexpr int BK = KIND == MM_F16 ? 64 : KIND == MM_TF32 ? 32 : 128, PARTS = KIND == MM_TF32 ? 2 : 1; };
 
-template <class T> struct BmParams {
+// A product of a launch.  Its units (tiles x splits) follow those of the product before; a CTA (or pair) takes every step-th unit of the launch.
+template <class T> struct BmJob {
     T *C, *g, *u, *dg, *du;
     const T *bias; const float *xs, *ws;
     uint32_t *part;
-    int N, M, tiles_m, tiles_n, tiles, kps, ksteps, splits, stages, a_mn, b_mn, vec;       // kps: K steps of a term
+    int N, M, tiles_m, tiles_n, kps, ksteps, splits, first, a_mn, b_mn, vec;               // kps: K steps of a term
+};
+static constexpr int BM_JOBS = 4;
+constexpr int bm_jobs(int epi) { return epi == FFN_PLAIN ? BM_JOBS : 1; }
+template <class T, int JOBS> struct BmParams {
+    BmJob<T> job[JOBS];
+    int jobs, units, stages;
     uint32_t stage_bytes;
     int *status;
 };
 struct BmMaps { CUtensorMap a[2], b[2]; };
+template <int JOBS> struct BmMapList { BmMaps of[JOBS]; };
 
 // D = A B^T of 8-bit integers, 32 bytes of K
 template <bool PAIR> __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
@@ -172,7 +180,7 @@ template <class T, int W> struct BmTile {
 };
 // The results of W columns from col on of the 32 rows from row0 on.  v: the accumulators (gate), w: the second ones (up); gq, uq: G and U as BmTile::fetch left them.
 template <class T, int EPI, int W>
-__device__ __forceinline__ void bm_tile_results(const BmParams<T> &p, int row0, int col, float (&v)[W], float (&w)[W], const uint4 (&gq)[BmTile<T, W>::CHUNKS],
+__device__ __forceinline__ void bm_tile_results(const BmJob<T> &p, int row0, int col, float (&v)[W], float (&w)[W], const uint4 (&gq)[BmTile<T, W>::CHUNKS],
                                                 const uint4 (&uq)[BmTile<T, W>::CHUNKS], unsigned char *stage, int lane)
 {
     typedef BmTile<T, W> Tile;
@@ -208,7 +216,7 @@ __device__ __forceinline__ void bm_tile_results(const BmParams<T> &p, int row0, 
     Tile::store(p.C + at, p.M, rows, cols, vec, v, stage, lane);
 }
 // The same for four columns of a row (from partial tiles)
-template <class T, int EPI> __device__ __forceinline__ void bm_results(const BmParams<T> &p, int row, int col, float (&v)[4], float (&w)[4])
+template <class T, int EPI> __device__ __forceinline__ void bm_results(const BmJob<T> &p, int row, int col, float (&v)[4], float (&w)[4])
 {
     constexpr bool FAST = sizeof(T) == 2;
     const size_t at = (size_t)row * p.M + col;
@@ -232,14 +240,29 @@ template <class T, int EPI> __device__ __forceinline__ void bm_results(const BmP
 }
 
 // tile -> row block, column block: eight row blocks share a sweep over the columns
-template <class T> __device__ __forceinline__ void bm_locate(const BmParams<T> &p, int tile, int &rb, int &cb)
+template <class T> __device__ __forceinline__ void bm_locate(const BmJob<T> &p, int tile, int &rb, int &cb)
 {
     const int g = tile / (8 * p.tiles_m), in = tile - g * 8 * p.tiles_m, rows = min(8, p.tiles_n - 8 * g);
     rb = 8 * g + in % rows; cb = in / rows;
 }
 
+// unit of a launch -> product, tile, part of its K
+struct BmUnit { int job, tile, rank, ks0, ks1; };
+template <class T, int JOBS> __device__ __forceinline__ BmUnit bm_unit(const BmParams<T, JOBS> &p, int unit)
+{
+    BmUnit u;
+    u.job = 0;
+#pragma unroll
+    for (int i = 1; i < JOBS; i++) if (i < p.jobs && unit >= p.job[i].first) u.job = i;
+    const BmJob<T> &j = p.job[u.job];
+    unit -= j.first;
+    u.tile = unit / j.splits; u.rank = unit - u.tile * j.splits;
+    u.ks0 = j.ksteps * u.rank / j.splits; u.ks1 = j.ksteps * (u.rank + 1) / j.splits;
+    return u;
+}
+
 template <int KIND, class T, int EPI, int BN, bool PAIR>
-__global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_constant__ BmMaps maps, const __grid_constant__ BmParams<T> p)
+__global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_constant__ BmMapList<bm_jobs(EPI)> maps, const __grid_constant__ BmParams<T, bm_jobs(EPI)> p)
 {
     pdl_wait();
     constexpr int BK = BmCfg<KIND>::BK, PARTS = BmCfg<KIND>::PARTS;
@@ -261,8 +284,7 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int ST = p.stages;
-    const int group = PAIR ? 2 : p.splits, rank = (int)blockIdx.x % group, first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
-    const int ks0 = PAIR ? 0 : p.ksteps * rank / p.splits, ks1 = PAIR ? p.ksteps : p.ksteps * (rank + 1) / p.splits;
+    const int rank = PAIR ? (int)blockIdx.x % 2 : 0, first = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x, step = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
     const int row_of_tile = PAIR ? rank * BM_ROWS : 0;
 
     if (tid == 0) {
@@ -271,7 +293,7 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
         mbar_init(&last_bar, 1);
         failed_s = 0;
         fence_barrier_init();
-        tma_prefetch_desc(&maps.a[0]); tma_prefetch_desc(&maps.b[0]);
+        tma_prefetch_desc(&maps.of[0].a[0]); tma_prefetch_desc(&maps.of[0].b[0]);
     }
     if (warp == 0) {
         if constexpr (PAIR) {
@@ -290,12 +312,15 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
         int s = 0;
         uint32_t phase = 1, issued = 0;                                             // the first pass over the ring finds it empty
         bool ok = true;
-        for (int tile = first; tile < p.tiles && ok; tile += step) {
+        for (int unit = first; unit < p.units && ok; unit += step) {
+            const BmUnit un = bm_unit(p, unit);
+            const BmJob<T> &j = p.job[un.job];
+            const BmMaps &map = maps.of[un.job];
             int rb, cb;
-            bm_locate(p, tile, rb, cb);
+            bm_locate(j, un.tile, rb, cb);
             const int row0 = rb * ROWS + row_of_tile, col0 = cb * BNC;
-            int term = ks0 / p.kps, kt = ks0 - term * p.kps;
-            for (int k = ks0; k < ks1; k++) {
+            int term = un.ks0 / j.kps, kt = un.ks0 - term * j.kps;
+            for (int k = un.ks0; k < un.ks1; k++) {
                 if (!tm_wait(&empty[s], phase, failed)) { ok = false; break; }
                 if (elect_one()) {
                     const uint32_t st = sbase + s * p.stage_bytes, sb = st + PARTS * A_BYTES;
@@ -305,27 +330,27 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                         else tma_load_3d(dst, m, &full[s], x, y, z);
                     };
                     if (!PAIR || rank == 0) mbar_arrive_expect_tx(&full[s], PAIR ? 2 * p.stage_bytes : p.stage_bytes);
-                    const CUtensorMap *ma = &maps.a[term], *mb = &maps.b[EPI == FFN_GATE ? 0 : term];
+                    const CUtensorMap *ma = &map.a[term], *mb = &map.b[EPI == FFN_GATE ? 0 : term];
 #pragma unroll
                     for (int z = 0; z < PARTS; z++) {
-                        if (KIND == MM_F16 && p.a_mn) { for (int j = 0; j < 2; j++) load(st + j * 8192u, ma, row0 + 64 * j, kt * BK, 0); }
+                        if (KIND == MM_F16 && j.a_mn) { for (int q = 0; q < 2; q++) load(st + q * 8192u, ma, row0 + 64 * q, kt * BK, 0); }
                         else load(st + z * A_BYTES, ma, kt * BK, row0, z);
                         if constexpr (EPI == FFN_GATE) {
-                            if constexpr (PAIR) load(sb, &maps.b[rank], kt * BK, col0, 0);
+                            if constexpr (PAIR) load(sb, &map.b[rank], kt * BK, col0, 0);
                             else {
-                                load(sb + z * B_BYTES, &maps.b[0], kt * BK, col0, z);
-                                load(sb + z * B_BYTES + B_BYTES / 2, &maps.b[1], kt * BK, col0, z);
+                                load(sb + z * B_BYTES, &map.b[0], kt * BK, col0, z);
+                                load(sb + z * B_BYTES + B_BYTES / 2, &map.b[1], kt * BK, col0, z);
                             }
                         } else {
                             const int c = col0 + (PAIR ? rank * BNL : 0);
-                            if (KIND == MM_F16 && p.b_mn) { for (int j = 0; j < BNL / 64; j++) load(sb + j * 8192u, mb, c + 64 * j, kt * BK, 0); }
+                            if (KIND == MM_F16 && j.b_mn) { for (int q = 0; q < BNL / 64; q++) load(sb + q * 8192u, mb, c + 64 * q, kt * BK, 0); }
                             else load(sb + z * B_BYTES, mb, kt * BK, c, z);
                         }
                     }
                 }
                 __syncwarp();
                 issued++;
-                if (++kt == p.kps) { kt = 0; term++; }
+                if (++kt == j.kps) { kt = 0; term++; }
                 if (++s == ST) { s = 0; phase ^= 1u; }
             }
         }
@@ -338,19 +363,21 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
             }
     } else if (warp == BM_EPI + 1) {
         if (!PAIR || rank == 0) {
-            const uint32_t majors = (p.a_mn ? IDESC_A_MN_MAJOR : 0u) | (p.b_mn ? IDESC_B_MN_MAJOR : 0u);
-            const uint32_t idesc = KIND == MM_F16 ? (mma_idesc(FMT_F16, ROWS, BN) | majors) : KIND == MM_I8 ? i8_idesc(ROWS, BN) : mma_idesc(FMT_TF32, ROWS, 2 * BN);
             const uint32_t idesc_lo = mma_idesc(FMT_TF32, ROWS, BN);
-            // descriptor words that do not depend on the stage, and the step of one MMA (32 bytes or 16 rows of K) in 16-byte units
-            const uint64_t desc_a = KIND == MM_F16 && p.a_mn ? smem_desc_swizzled(0, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(0, 1024);
-            const uint64_t desc_b = KIND == MM_F16 && p.b_mn ? smem_desc_swizzled(0, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(0, 1024);
-            const uint32_t step_a = KIND == MM_F16 && p.a_mn ? 128u : 2u, step_b = KIND == MM_F16 && p.b_mn ? 128u : 2u;
             int s = 0, it = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int tile = first; tile < p.tiles && ok; tile += step)
-                for (int kc = ks0; kc < ks1 && ok; it++) {
-                    const int kend = KIND == MM_TF32 ? min(ks1, kc + BM_CHUNK) : ks1, buf = it % NBUF, use = it / NBUF;
+            for (int unit = first; unit < p.units && ok; unit += step) {
+                const BmUnit un = bm_unit(p, unit);
+                const bool a_mn = KIND == MM_F16 && p.job[un.job].a_mn, b_mn = KIND == MM_F16 && p.job[un.job].b_mn;
+                const uint32_t majors = (a_mn ? IDESC_A_MN_MAJOR : 0u) | (b_mn ? IDESC_B_MN_MAJOR : 0u);
+                const uint32_t idesc = KIND == MM_F16 ? (mma_idesc(FMT_F16, ROWS, BN) | majors) : KIND == MM_I8 ? i8_idesc(ROWS, BN) : mma_idesc(FMT_TF32, ROWS, 2 * BN);
+                // descriptor words that do not depend on the stage, and the step of one MMA (32 bytes or 16 rows of K) in 16-byte units
+                const uint64_t desc_a = a_mn ? smem_desc_swizzled(0, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(0, 1024);
+                const uint64_t desc_b = b_mn ? smem_desc_swizzled(0, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(0, 1024);
+                const uint32_t step_a = a_mn ? 128u : 2u, step_b = b_mn ? 128u : 2u;
+                for (int kc = un.ks0; kc < un.ks1 && ok; it++) {
+                    const int kend = KIND == MM_TF32 ? min(un.ks1, kc + BM_CHUNK) : un.ks1, buf = it % NBUF, use = it / NBUF;
                     if (use > 0 && !tm_wait(&acc_empty[buf], (uint32_t)(use - 1) & 1u, failed)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t d = tmem + buf * BUF_COLS;
@@ -376,6 +403,7 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                     if (ok && elect_one()) tm_commit<PAIR>(&acc_full[buf]);
                     __syncwarp();
                 }
+            }
             if (!ok) {                                                              // given up: what was issued ends first
                 if (elect_one()) tm_commit<PAIR>(&last_bar);
                 __syncwarp();
@@ -391,13 +419,16 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
         typedef BmTile<T, W> Tile;
         int it = 0;
         bool ok = true;
-        for (int tile = first; tile < p.tiles && ok; tile += step) {
+        for (int unit = first; unit < p.units && ok; unit += step) {
+            const BmUnit un = bm_unit(p, unit);
+            const BmJob<T> &j = p.job[un.job];
+            const int ks0 = un.ks0, ks1 = un.ks1;
             int rb, cb;
-            bm_locate(p, tile, rb, cb);
+            bm_locate(j, un.tile, rb, cb);
             const int row0 = rb * ROWS + row_of_tile + quarter * 32, col0 = cb * BNC + half * CW;
             constexpr int NS = KIND == MM_TF32 ? CW : 1, NS2 = KIND == MM_TF32 && EPI == FFN_GATE ? CW : 1;
             float sum[NS], sum2[NS2];
-            const bool whole = PAIR || p.splits == 1;                               // results leave from here, not partial tiles
+            const bool whole = PAIR || j.splits == 1;                               // results leave from here, not partial tiles
             auto take = [&](uint32_t d, int c, float (&v)[W]) {                     // W accumulators of this lane's row
                 uint32_t a[W];
                 if constexpr (W == 32) tmem_ld32w(d + c, a); else tmem_ld16w(d + c, a);
@@ -406,11 +437,11 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                     if constexpr (W == 32) { tmem_ld32w(d + BN + c, b); tmem_ld32w(d + 2 * BN + c, x); } else { tmem_ld16w(d + BN + c, b); tmem_ld16w(d + 2 * BN + c, x); }
                     tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < W; j++) v[j] = __uint_as_float(a[j]) + (__uint_as_float(b[j]) + __uint_as_float(x[j]));
+                    for (int q = 0; q < W; q++) v[q] = __uint_as_float(a[q]) + (__uint_as_float(b[q]) + __uint_as_float(x[q]));
                 } else {
                     tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < W; j++) v[j] = KIND == MM_I8 && whole ? (float)(int)a[j] : __uint_as_float(a[j]);
+                    for (int q = 0; q < W; q++) v[q] = KIND == MM_I8 && whole ? (float)(int)a[q] : __uint_as_float(a[q]);
                 }
             };
             auto release = [&](int buf) {                                           // the accumulators are in registers: they may be overwritten
@@ -425,35 +456,35 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                 tc_fence_after();
                 return there;
             };
-            uint4 gq[Tile::CHUNKS], uq[Tile::CHUNKS], gn[Tile::CHUNKS], un[Tile::CHUNKS];       // G and U of this piece and the next
+            uint4 gq[Tile::CHUNKS], uq[Tile::CHUNKS], g1[Tile::CHUNKS], u1[Tile::CHUNKS];       // G and U of this piece and the next
             auto fetch = [&](int c) {
                 if constexpr (EPI == FFN_GATE_BW) {
-                    if (!whole || row0 >= p.N || c >= CW || col0 + c >= p.M) return;
-                    const size_t at = (size_t)row0 * p.M + col0 + c;
-                    Tile::fetch(p.g + at, p.M, p.N - row0, p.M - col0 - c, p.vec, gn, lane);
-                    Tile::fetch(p.u + at, p.M, p.N - row0, p.M - col0 - c, p.vec, un, lane);
+                    if (!whole || row0 >= j.N || c >= CW || col0 + c >= j.M) return;
+                    const size_t at = (size_t)row0 * j.M + col0 + c;
+                    Tile::fetch(j.g + at, j.M, j.N - row0, j.M - col0 - c, j.vec, g1, lane);
+                    Tile::fetch(j.u + at, j.M, j.N - row0, j.M - col0 - c, j.vec, u1, lane);
                 }
             };
-            uint32_t *mine = p.part + ((size_t)(tile * p.splits + rank) * BM_ROWS + row_in) * BN;        // row of the partial tile (splits > 1)
+            uint32_t *mine = j.part + ((size_t)(un.tile * j.splits + un.rank) * BM_ROWS + row_in) * BN;        // row of the partial tile (splits > 1)
             auto leave = [&](int c, float (&v)[W], float (&w)[W]) {
                 if (!whole) {
 #pragma unroll
-                    for (int j = 0; j < W; j += 4) {
-                        *reinterpret_cast<float4 *>(mine + half * CW + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                        if constexpr (EPI == FFN_GATE) *reinterpret_cast<float4 *>(mine + BNC + half * CW + c + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+                    for (int q = 0; q < W; q += 4) {
+                        *reinterpret_cast<float4 *>(mine + half * CW + c + q) = make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+                        if constexpr (EPI == FFN_GATE) *reinterpret_cast<float4 *>(mine + BNC + half * CW + c + q) = make_float4(w[q], w[q + 1], w[q + 2], w[q + 3]);
                     }
-                } else if (row0 < p.N && col0 + c < p.M) bm_tile_results<T, EPI, W>(p, row0, col0 + c, v, w, gq, uq, stage, lane);
+                } else if (row0 < j.N && col0 + c < j.M) bm_tile_results<T, EPI, W>(j, row0, col0 + c, v, w, gq, uq, stage, lane);
             };
             auto turn_over = [&]() {
 #pragma unroll
-                for (int i = 0; i < Tile::CHUNKS; i++) { gq[i] = gn[i]; uq[i] = un[i]; }
+                for (int i = 0; i < Tile::CHUNKS; i++) { gq[i] = g1[i]; uq[i] = u1[i]; }
             };
             fetch(0);
             if constexpr (KIND == MM_TF32) {
 #pragma unroll
-                for (int j = 0; j < NS; j++) sum[j] = 0.f;
+                for (int q = 0; q < NS; q++) sum[q] = 0.f;
 #pragma unroll
-                for (int j = 0; j < NS2; j++) sum2[j] = 0.f;
+                for (int q = 0; q < NS2; q++) sum2[q] = 0.f;
                 for (int kc = ks0; kc < ks1; kc += BM_CHUNK, it++) {
                     const int buf = it % NBUF, use = it / NBUF;
                     if (!arrived(buf, use)) { ok = false; break; }
@@ -463,11 +494,11 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                         float v[W];
                         take(d, half * CW + c, v);
 #pragma unroll
-                        for (int j = 0; j < W; j++) sum[c + j] += v[j];
+                        for (int q = 0; q < W; q++) sum[c + q] += v[q];
                         if constexpr (EPI == FFN_GATE) {
                             take(d, BNC + half * CW + c, v);
 #pragma unroll
-                            for (int j = 0; j < W; j++) sum2[c + j] += v[j];
+                            for (int q = 0; q < W; q++) sum2[c + q] += v[q];
                         }
                     }
                     release(buf);
@@ -477,7 +508,7 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                 for (int c = 0; c < CW; c += W) {
                     float v[W], w[W];
 #pragma unroll
-                    for (int j = 0; j < W; j++) { v[j] = sum[c + j]; w[j] = EPI == FFN_GATE ? sum2[EPI == FFN_GATE ? c + j : 0] : 0.f; }
+                    for (int q = 0; q < W; q++) { v[q] = sum[c + q]; w[q] = EPI == FFN_GATE ? sum2[EPI == FFN_GATE ? c + q : 0] : 0.f; }
                     turn_over();
                     fetch(c + W);
                     leave(c, v, w);
@@ -526,7 +557,7 @@ template <int KIND, int BN> __device__ __forceinline__ void bm_add_parts(const u
     }
 }
 // The results from the partial tiles of a split contraction: a thread per four neighbouring results, partial tiles added in order.
-template <int KIND, class T, int EPI, int BN> __global__ void __launch_bounds__(256) bm_reduce_kernel(const __grid_constant__ BmParams<T> p)
+template <int KIND, class T, int EPI, int BN> __global__ void __launch_bounds__(256) bm_reduce_kernel(const __grid_constant__ BmJob<T> p)
 {
     pdl_wait();
     constexpr int BNC = EPI == FFN_GATE ? BN / 2 : BN, QUADS = BNC / 4, PER = BM_ROWS * QUADS;       // (PER is a multiple of 256: a block stays inside one tile)
@@ -556,30 +587,41 @@ static bool bm_map(CUtensorMap *m, CUtensorMapDataType type, int esize, const vo
 // Tile and CTAs per tile with the fewest cycles by the model that the plain products use (tl_gemm_tma.cu): a K step costs its tensor time or
 // what its bytes take from L2 into an SM (58 bytes per cycle with every SM loading, 81 with half of them), a pair's a third more than its tensor
 // time; a tile 2500 cycles beside its K steps, a launch 2000 (pairs 10000), partial tiles a launch and their bytes.
-struct BmPlan { int BN, pair, splits; };
-static BmPlan bm_plan(int kind, int epi, int N, int M, int ksteps)
+struct BmPlan { int BN, pair; };
+// Several products in one launch: the sum of their units' cycles over the CTAs and the longest unit, for which a product's K is split while CTAs are idle.
+template <class T, int JOBS> static BmPlan bm_plan(int kind, int epi, BmParams<T, JOBS> &p)
 {
-    BmPlan plan = {64, 0, 1};
+    BmPlan plan = {64, 0};
     double best = 1e30;
     const int bns[4] = {256, 128, 64, 256};
     for (int i = kind == MM_TF32 ? 1 : 0; i < (kind == MM_TF32 ? 3 : 4); i++) {
         const bool two = i == 3;
-        const int bn = bns[i], bnc = epi == FFN_GATE ? bn / 2 : bn;
-        const long long tiles = (long long)ceil_div(N, two ? 256 : 128) * ceil_div(M, bnc);
-        for (int s = 1; s <= (two ? 1 : 16); s++) {
-            if (s > 1 && (ksteps < 2 * s || tiles * s > sm_count())) break;
-            const long long ctas = tiles * s * (two ? 2 : 1);
-            const double tensor = (kind == MM_TF32 ? 6.0 : 2.0) * bn * (two ? 4.0 / 3.0 : 1.0);
-            const double fill = (kind == MM_TF32 ? 2 : 1) * 128.0 * (128 + (two ? bn / 2 : bn)) / (ctas <= sm_count() / 2 ? 81.0 : 58.0);
-            const double reduce = s > 1 ? 4000.0 + 512.0 * bn * tiles * s / 2000.0 : 0.0;
-            const double cost = (two ? 10000.0 : 2000.0) + (double)ceil_div(ctas, sm_count()) * (std::max(tensor, fill) * ceil_div(ksteps, s) + 2500.0) + reduce;
-            if (cost < 0.97 * best) { best = cost; plan = {bn, two ? 1 : 0, s}; }
+        const int bn = bns[i], bnc = epi == FFN_GATE ? bn / 2 : bn, places = two ? sm_count() / 2 : sm_count();
+        int splits[JOBS], tiles[JOBS], units = 0;
+        for (int k = 0; k < p.jobs; k++) { splits[k] = 1; units += tiles[k] = ceil_div(p.job[k].N, two ? 256 : 128) * ceil_div(p.job[k].M, bnc); }
+        const double tensor = (kind == MM_TF32 ? 6.0 : 2.0) * bn * (two ? 4.0 / 3.0 : 1.0);
+        for (;;) {
+            const double fill = (kind == MM_TF32 ? 2 : 1) * 128.0 * (128 + (two ? bn / 2 : bn)) / (units <= places / 2 ? 81.0 : 58.0), step = std::max(tensor, fill);
+            double sum = 0, longest = 0, reduce = 0;
+            int at = 0;
+            for (int k = 0; k < p.jobs; k++) {
+                const double unit = step * ceil_div(p.job[k].ksteps, splits[k]) + 2500.0;
+                sum += unit * tiles[k] * splits[k];
+                if (unit > longest) { longest = unit; at = k; }
+                if (splits[k] > 1) reduce += 4000.0 + 512.0 * bn * tiles[k] * splits[k] / 2000.0;
+            }
+            const double work = p.jobs == 1 ? ceil_div(units, places) * longest : std::max(sum / places + 0.3 * longest, longest);
+            const double cost = (two ? 10000.0 : 2000.0) + work + reduce;
+            if (cost < 0.97 * best) { best = cost; plan = {bn, two ? 1 : 0}; for (int k = 0; k < p.jobs; k++) p.job[k].splits = splits[k]; }
+            if (two || splits[at] >= 16 || units + tiles[at] > places || p.job[at].ksteps < 2 * (splits[at] + 1)) break;
+            splits[at]++;
+            units += tiles[at];
         }
     }
     return plan;
 }
 
-template <int KIND, class T, int EPI, int BN, bool PAIR> static void bm_launch(const BmMaps &maps, const BmParams<T> &p)
+template <int KIND, class T, int EPI, int BN, bool PAIR> static void bm_launch(const BmMapList<bm_jobs(EPI)> &maps, const BmParams<T, bm_jobs(EPI)> &p)
 {
     const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
     static bool attr_set = false;
@@ -587,13 +629,15 @@ template <int KIND, class T, int EPI, int BN, bool PAIR> static void bm_launch(c
         cudaFuncSetAttribute(block_mm_kernel<KIND, T, EPI, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(BM_RING + 1024));
         attr_set = true;
     }
-    if constexpr (PAIR) TL_LAUNCH_CLUSTER((block_mm_kernel<KIND, T, EPI, BN, PAIR>), (unsigned)(2 * std::min(p.tiles, sm_count() / 2)), BM_THREADS, smem, 2, maps, p);
+    if constexpr (PAIR) TL_LAUNCH_CLUSTER((block_mm_kernel<KIND, T, EPI, BN, PAIR>), (unsigned)(2 * std::min(p.units, sm_count() / 2)), BM_THREADS, smem, 2, maps, p);
     else {
-        TL_LAUNCH((block_mm_kernel<KIND, T, EPI, BN, PAIR>), (unsigned)(p.splits > 1 ? p.tiles * p.splits : std::min(p.tiles, sm_count())), BM_THREADS, smem, maps, p);
-        if (p.splits > 1) TL_LAUNCH((bm_reduce_kernel<KIND, T, EPI, BN>), (unsigned)((long long)p.tiles * BM_ROWS * (EPI == FFN_GATE ? BN / 2 : BN) / 4 / 256), 256, 0, p);
+        TL_LAUNCH((block_mm_kernel<KIND, T, EPI, BN, PAIR>), (unsigned)std::min(p.units, sm_count()), BM_THREADS, smem, maps, p);
+        for (int k = 0; k < p.jobs; k++)
+            if (p.job[k].splits > 1)
+                TL_LAUNCH((bm_reduce_kernel<KIND, T, EPI, BN>), (unsigned)((long long)p.job[k].tiles_m * p.job[k].tiles_n * BM_ROWS * (EPI == FFN_GATE ? BN / 2 : BN) / 4 / 256), 256, 0, p.job[k]);
     }
 }
-template <int KIND, class T, int EPI> static void bm_dispatch(const BmPlan &plan, const BmMaps &maps, const BmParams<T> &p)
+template <int KIND, class T, int EPI> static void bm_dispatch(const BmPlan &plan, const BmMapList<bm_jobs(EPI)> &maps, const BmParams<T, bm_jobs(EPI)> &p)
 {
     if constexpr (KIND != MM_TF32) {
         if (plan.pair) return bm_launch<KIND, T, EPI, 256, true>(maps, p);
@@ -603,15 +647,20 @@ template <int KIND, class T, int EPI> static void bm_dispatch(const BmPlan &plan
     else bm_launch<KIND, T, EPI, 64, false>(maps, p);
 }
 // what does not depend on the operands' layout; false: no memory for the partial tiles
-template <int KIND, class T, int EPI> static bool bm_setup(Scope &sc, const BmPlan &plan, BmParams<T> &p)
+template <int KIND, class T, int EPI> static bool bm_setup(Scope &sc, const BmPlan &plan, BmParams<T, bm_jobs(EPI)> &p)
 {
     const int bnc = EPI == FFN_GATE ? plan.BN / 2 : plan.BN;
     p.status = tc_status_word();
-    p.splits = plan.splits;
-    p.tiles_m = ceil_div(p.M, bnc); p.tiles_n = ceil_div(p.N, plan.pair ? 2 * BM_ROWS : BM_ROWS); p.tiles = p.tiles_m * p.tiles_n;
     p.stage_bytes = BmCfg<KIND>::PARTS * (BM_ROWS * 128u + (uint32_t)(plan.pair ? plan.BN / 2 : plan.BN) * 128u);
     p.stages = std::min<int>(BM_MAX_STAGES, BM_RING / p.stage_bytes);
-    if (p.splits > 1 && !(p.part = sc.scratch<uint32_t>((size_t)p.tiles * p.splits * BM_ROWS * plan.BN))) return false;
+    p.units = 0;
+    for (int k = 0; k < p.jobs; k++) {
+        BmJob<T> &j = p.job[k];
+        j.tiles_m = ceil_div(j.M, bnc); j.tiles_n = ceil_div(j.N, plan.pair ? 2 * BM_ROWS : BM_ROWS);
+        j.first = p.units;
+        p.units += j.tiles_m * j.tiles_n * j.splits;
+        if (j.splits > 1 && !(j.part = sc.scratch<uint32_t>((size_t)j.tiles_m * j.tiles_n * j.splits * BM_ROWS * plan.BN))) return false;
+    }
     return p.status != nullptr;
 }
 
@@ -626,83 +675,104 @@ static bool bm_no_map()
     set_error(TL_ERR_CUDA, "cuTensorMapEncodeTiled refused an operand");
     return false;
 }
-template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> &f)
+// copies of up to twelve operands in one launch
+template <class T> struct BmPacks { PackOp<T> op[12]; int count, blocks; };
+template <class T> __global__ void __launch_bounds__(256) bm_pack_kernel(const __grid_constant__ BmPacks<T> ops)
 {
-    constexpr int KIND = sizeof(T) == 2 ? MM_F16 : MM_TF32, BK = BmCfg<KIND>::BK;
+    pdl_wait();
+    int k = 0;
+    while (k + 1 < ops.count && (int)blockIdx.x >= ops.op[k + 1].first) k++;
+    pack_kmajor_block<T>(ops.op[k]);
+}
+template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> *list, int count)
+{
+    constexpr int KIND = sizeof(T) == 2 ? MM_F16 : MM_TF32, BK = BmCfg<KIND>::BK, JOBS = bm_jobs(EPI);
     constexpr long long EB = 16 / (long long)sizeof(T);
     if (!bm_ready()) return false;
-    const int nb = EPI == FFN_GATE ? 2 : f.terms, Kp = (int)(((long long)f.K + EB - 1) / EB * EB);
+    // what takes longest goes first
+    const FfnProduct<T> *order[JOBS];
+    for (int k = 0; k < count; k++) order[k] = list + k;
+    std::sort(order, order + count, [](const FfnProduct<T> *x, const FfnProduct<T> *y) { return (long long)x->K * x->terms > (long long)y->K * y->terms; });
     struct Op { const T *at; long long os, ps; int mn; };
-    PackOps<T> pack[2];                                                              // a launch packs two operands at most
-    int blocks[2] = {0, 0}, packs = 0;
-    pack[0].count = pack[1].count = 0;
-    // one layout for all operands of a side: they share strides, and all are read in place or none
-    auto side = [&](const T *const *src, int count, long long rs, long long cs, int rows, Op *o) -> bool {
-        int where = tm_in_place<T>(src[0], rs, cs, 0, rows, f.K, 1);
-        if (count > 1 && tm_in_place<T>(src[1], rs, cs, 0, rows, f.K, 1) != where) where = 0;
-        for (int i = 0; i < count; i++) {
+    struct Done { const T *src; long long rs, cs; int rows, K; Op op; } done[12];
+    BmPacks<T> pack;
+    pack.count = pack.blocks = 0;
+    // one layout for all operands of a side: they share strides, and all are read in place or none.  An operand of two products is copied once.
+    auto side = [&](const T *const *src, int n, long long rs, long long cs, int rows, int K, Op *o) -> bool {
+        const int Kp = (int)(((long long)K + EB - 1) / EB * EB);
+        int where = tm_in_place<T>(src[0], rs, cs, 0, rows, K, 1);
+        if (n > 1 && tm_in_place<T>(src[1], rs, cs, 0, rows, K, 1) != where) where = 0;
+        for (int i = 0; i < n; i++) {
             if (where) { o[i] = {src[i], where == 1 ? rs : cs, 0, where - 1}; continue; }
+            int k = 0;
+            while (k < pack.count && !(done[k].src == src[i] && done[k].rs == rs && done[k].cs == cs && done[k].rows == rows && done[k].K == K)) k++;
+            if (k < pack.count) { o[i] = done[k].op; continue; }
             const size_t size = ((size_t)rows * Kp + 63) & ~(size_t)63;
             T *hi = sc.scratch<T>(BmCfg<KIND>::PARTS * size);
             if (!hi) return false;
-            PackOps<T> &q = pack[packs / 2];
-            int &nb_ = blocks[packs / 2];
-            packs++;
             const bool straight = cs == 1;
-            PackOp<T> &op = q.op[q.count++];
-            op = {src[i], hi, sizeof(T) == 4 ? hi + size : nullptr, rs, cs, 0, rows, f.K, Kp, ceil_div(Kp, straight ? 64 : 32), ceil_div(rows, straight ? 32 : 64), nb_, straight,
+            PackOp<T> &op = pack.op[pack.count];
+            op = {src[i], hi, sizeof(T) == 4 ? hi + size : nullptr, rs, cs, 0, rows, K, Kp, ceil_div(Kp, straight ? 64 : 32), ceil_div(rows, straight ? 32 : 64), pack.blocks, straight,
                   (straight ? rs : rs == 1 ? cs : 1) % EB == 0 && ((uintptr_t)src[i] & 15) == 0};
-            nb_ += op.nk * op.nr;
+            pack.blocks += op.nk * op.nr;
             o[i] = {hi, Kp, (long long)size, 0};
+            done[pack.count++] = {src[i], rs, cs, rows, K, o[i]};
         }
         return true;
     };
-    Op a[2], b[2];
-    if (!side(f.A, f.terms, f.a_rs, f.a_cs, f.N, a) || !side(f.B, nb, f.b_cs, f.b_rs, f.M, b)) return false;
-    BmParams<T> p = {};
-    p.C = f.C; p.g = f.g; p.u = f.u; p.dg = f.dg; p.du = f.du; p.N = f.N; p.M = f.M;
-    p.kps = ceil_div(f.K, BK); p.ksteps = p.kps * f.terms;
-    p.a_mn = a[0].mn; p.b_mn = b[0].mn;
+    Op a[JOBS][2], b[JOBS][2];
+    BmParams<T, JOBS> p = {};
+    p.jobs = count;
     auto odd = [](const void *q) { return ((uintptr_t)q & 15) != 0; };
-    p.vec = f.M % EB == 0 && !odd(f.C) && !odd(f.g) && !odd(f.u) && !odd(f.dg) && !odd(f.du);
-    const BmPlan plan = bm_plan(KIND, EPI, f.N, f.M, p.ksteps);
+    for (int k = 0; k < count; k++) {
+        const FfnProduct<T> &f = *order[k];
+        BmJob<T> &j = p.job[k];
+        if (!side(f.A, f.terms, f.a_rs, f.a_cs, f.N, f.K, a[k]) || !side(f.B, EPI == FFN_GATE ? 2 : f.terms, f.b_cs, f.b_rs, f.M, f.K, b[k])) return false;
+        j.C = f.C; j.g = f.g; j.u = f.u; j.dg = f.dg; j.du = f.du; j.N = f.N; j.M = f.M;
+        j.kps = ceil_div(f.K, BK); j.ksteps = j.kps * f.terms;
+        j.a_mn = a[k][0].mn; j.b_mn = b[k][0].mn;
+        j.vec = f.M % EB == 0 && !odd(f.C) && !odd(f.g) && !odd(f.u) && !odd(f.dg) && !odd(f.du);
+    }
+    const BmPlan plan = bm_plan<T, JOBS>(KIND, EPI, p);
     if (!bm_setup<KIND, T, EPI>(sc, plan, p)) return false;
     const CUtensorMapDataType type = sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-    auto map_of = [&](CUtensorMap *m, const Op &o, int rows, int box_rows) -> bool {
-        return o.mn ? bm_map(m, type, (int)sizeof(T), o.at, rows, f.K, 1, o.os, 0, 64, 64) : bm_map(m, type, sizeof(T), o.at, f.K, rows, BmCfg<KIND>::PARTS, o.os, o.ps, BK, box_rows);
-    };
-    BmMaps maps;
-    const int b_rows = EPI == FFN_GATE ? plan.BN / 2 : plan.pair ? plan.BN / 2 : plan.BN;
-    for (int i = 0; i < 2; i++) {
-        if (!map_of(&maps.a[i], a[std::min(i, f.terms - 1)], f.N, BM_ROWS) || !map_of(&maps.b[i], b[std::min(i, nb - 1)], f.M, b_rows)) return bm_no_map();
+    BmMapList<JOBS> maps;
+    const int b_rows = EPI == FFN_GATE || plan.pair ? plan.BN / 2 : plan.BN;
+    for (int k = 0; k < count; k++) {
+        const FfnProduct<T> &f = *order[k];
+        auto map_of = [&](CUtensorMap *m, const Op &o, int rows, int box_rows) -> bool {
+            return o.mn ? bm_map(m, type, (int)sizeof(T), o.at, rows, f.K, 1, o.os, 0, 64, 64) : bm_map(m, type, (int)sizeof(T), o.at, f.K, rows, BmCfg<KIND>::PARTS, o.os, o.ps, BK, box_rows);
+        };
+        for (int i = 0; i < f.terms; i++) if (!map_of(&maps.of[k].a[i], a[k][i], f.N, BM_ROWS)) return bm_no_map();
+        for (int i = 0; i < (EPI == FFN_GATE ? 2 : f.terms); i++) if (!map_of(&maps.of[k].b[i], b[k][i], f.M, b_rows)) return bm_no_map();
     }
-    for (int i = 0; i < 2; i++) if (pack[i].count) TL_LAUNCH((pack_kmajor_kernel<T>), blocks[i], 256, 0, pack[i]);
+    if (pack.count) TL_LAUNCH((bm_pack_kernel<T>), pack.blocks, 256, 0, pack);
     bm_dispatch<KIND, T, EPI>(plan, maps, p);
     return true;
 }
 #define INST(T)                                                             \
-    template bool block_mm<T, FFN_PLAIN>(Scope &, const FfnProduct<T> &);   \
-    template bool block_mm<T, FFN_GATE>(Scope &, const FfnProduct<T> &);    \
-    template bool block_mm<T, FFN_GATE_BW>(Scope &, const FfnProduct<T> &);
+    template bool block_mm<T, FFN_PLAIN>(Scope &, const FfnProduct<T> *, int);   \
+    template bool block_mm<T, FFN_GATE>(Scope &, const FfnProduct<T> *, int);    \
+    template bool block_mm<T, FFN_GATE_BW>(Scope &, const FfnProduct<T> *, int);
 INST(float)
 INST(__half)
 
-// rows of `size` bytes that do not lie on 16-byte boundaries -> rows of `padded` bytes (behind the end: never read); a thread per 16 bytes
-__global__ void __launch_bounds__(256) pack_rows_int8_kernel(const signed char *__restrict__ src, uint4 *__restrict__ dst, int rows, int size, int quads)
+// Rows of `size` bytes that do not lie on 16-byte boundaries -> rows of `quads` 16-byte groups (behind the end: never read), of both operands; a thread per group
+struct BmRows { const signed char *src[2]; uint4 *dst[2]; long long groups[2]; };
+__global__ void __launch_bounds__(256) pack_rows_int8_kernel(const __grid_constant__ BmRows p, int size, int quads)
 {
     pdl_wait();
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (e >= (long long)rows * quads) return;
-    const int r = (int)(e / quads), k = (int)(e - (long long)r * quads) * 16;
-    const signed char *s = src + (size_t)r * size + k;
-    uint32_t w[4];
+    long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int which = e >= p.groups[0];
+    if (which) e -= p.groups[0];
+    if (e >= p.groups[which]) return;
+    const long long r = e / quads;
+    const int k = (int)(e - r * quads) * 16;
+    const signed char *s = p.src[which] + (size_t)r * size + k;
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-        w[q] = 0;
-#pragma unroll
-        for (int b = 0; b < 4; b++) if (k + 4 * q + b < size) w[q] |= (uint32_t)(unsigned char)s[4 * q + b] << (8 * b);
-    }
-    dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int b = 0; b < 16; b++) if (k + b < size) w[b / 4] |= (uint32_t)(unsigned char)s[b] << (8 * (b % 4));
+    p.dst[which][e] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <class T> void linear_int8(Scope &sc, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out)
 {
@@ -716,19 +786,23 @@ template <class T> void linear_int8(Scope &sc, const signed char *x, const float
         if (in % 16 || ((uintptr_t)at[i] & 15)) {
             if (!(copy[i] = sc.scratch<signed char>((size_t)count[i] * quads * 16))) return;
         }
-    BmParams<T> p = {};
-    p.C = y; p.bias = bias; p.xs = xs; p.ws = ws; p.N = rows; p.M = out;
-    p.kps = p.ksteps = ceil_div(in, BmCfg<MM_I8>::BK);
-    p.vec = out % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)y & 15) == 0;
-    const BmPlan plan = bm_plan(MM_I8, FFN_INT8, rows, out, p.ksteps);
+    BmParams<T, 1> p = {};
+    BmJob<T> &j = p.job[0];
+    p.jobs = 1;
+    j.C = y; j.bias = bias; j.xs = xs; j.ws = ws; j.N = rows; j.M = out;
+    j.kps = j.ksteps = ceil_div(in, BmCfg<MM_I8>::BK);
+    j.vec = out % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)y & 15) == 0;
+    const BmPlan plan = bm_plan<T, 1>(MM_I8, FFN_INT8, p);
     if (!bm_setup<MM_I8, T, FFN_INT8>(sc, plan, p)) return;
-    BmMaps maps;
+    BmMapList<1> maps;
     for (int i = 0; i < 2; i++)
-        if (!bm_map(i ? &maps.b[0] : &maps.a[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, copy[i] ? copy[i] : at[i], in, count[i], 1, copy[i] ? (long long)quads * 16 : in, 0, BmCfg<MM_I8>::BK,
+        if (!bm_map(i ? &maps.of[0].b[0] : &maps.of[0].a[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, copy[i] ? copy[i] : at[i], in, count[i], 1, copy[i] ? (long long)quads * 16 : in, 0, BmCfg<MM_I8>::BK,
                     i ? (plan.pair ? plan.BN / 2 : plan.BN) : BM_ROWS)) { bm_no_map(); return; }
-    maps.a[1] = maps.a[0]; maps.b[1] = maps.b[0];
-    for (int i = 0; i < 2; i++)
-        if (copy[i]) TL_LAUNCH(pack_rows_int8_kernel, ceil_div((long long)count[i] * quads, 256), 256, 0, at[i], (uint4 *)copy[i], count[i], in, quads);
+    if (copy[0] || copy[1]) {
+        BmRows q;
+        for (int i = 0; i < 2; i++) { q.src[i] = at[i]; q.dst[i] = (uint4 *)copy[i]; q.groups[i] = copy[i] ? (long long)count[i] * quads : 0; }
+        TL_LAUNCH(pack_rows_int8_kernel, ceil_div(q.groups[0] + q.groups[1], 256), 256, 0, q, in, quads);
+    }
     bm_dispatch<MM_I8, T, FFN_INT8>(plan, maps, p);
 }
 template void linear_int8<float>(Scope &, const signed char *, const float *, const signed char *, const float *, const float *, float *, int, int, int);

@@ -31,7 +31,8 @@ template <class T> struct FfnProduct {
     long long a_rs, a_cs, b_rs, b_cs;
 };
 // On the tensor cores (tl_block_mm.cu); false: nothing launched, the error is set (no memory for an operand's copy, no tensor-map encoder)
-template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> &p);
+// FFN_PLAIN: up to four products in one launch, none of which may write what another one reads.
+template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> *list, int count);
 // Few tokens (FEW_ROWS at most), weights with K contiguous (tl_few_rows.cu): FFN_PLAIN of one term and FFN_GATE.  c_stride: elements between the rows of C.
 static constexpr int FEW_ROWS = 32;
 template <class T, int EPI> void few_rows_mm(Scope &sc, const FfnProduct<T> &p, long long c_stride);

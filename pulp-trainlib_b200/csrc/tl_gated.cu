@@ -27,12 +27,12 @@ template <class T> void gated_ffn_fw(Scope &sc, const GatedFfn<T> &f)
     p.A[0] = f.x; p.B[0] = f.wg; p.B[1] = f.wu; p.C = h; p.g = f.g; p.u = f.u; p.N = f.rows; p.M = f.hidden; p.K = f.in; p.terms = 1;
     p.a_rs = f.in; p.a_cs = 1; p.b_rs = 1; p.b_cs = f.in;
     if (few) few_rows_mm<T, FFN_GATE>(sc, p, pitch);
-    else if (!block_mm<T, FFN_GATE>(sc, p)) return;
+    else if (!block_mm<T, FFN_GATE>(sc, &p, 1)) return;
     FfnProduct<T> d = {};
     d.A[0] = h; d.B[0] = f.wd; d.C = f.y; d.N = f.rows; d.M = f.out; d.K = f.hidden; d.terms = 1;
     d.a_rs = pitch; d.a_cs = 1; d.b_rs = 1; d.b_cs = f.hidden;
     if (few) few_rows_mm<T, FFN_PLAIN>(sc, d, f.out);
-    else block_mm<T, FFN_PLAIN>(sc, d);
+    else block_mm<T, FFN_PLAIN>(sc, &d, 1);
 }
 template <class T> void gated_ffn_bw(Scope &sc, const GatedFfn<T> &f)
 {
@@ -43,23 +43,25 @@ template <class T> void gated_ffn_bw(Scope &sc, const GatedFfn<T> &f)
     p.A[0] = f.dy; p.B[0] = f.wd; p.C = h; p.g = f.g; p.u = f.u; p.dg = dg; p.du = du; p.N = f.rows; p.M = f.hidden; p.terms = 1;
     p.K = f.out; p.a_rs = f.out; p.a_cs = 1; p.b_rs = f.hidden; p.b_cs = 1;
     if (!f.dx && !f.dwg && !f.dwu) TL_LAUNCH((gate_kernel<T>), (unsigned)std::min<size_t>((n + 255) / 256, 16 * sm_count()), 256, 0, f.g, f.u, h, n);
-    else if (!block_mm<T, FFN_GATE_BW>(sc, p)) return;
+    else if (!block_mm<T, FFN_GATE_BW>(sc, &p, 1)) return;
+    // the gradients that are wanted, in one launch
+    FfnProduct<T> list[4];
+    int count = 0;
     if (f.dx) {
-        FfnProduct<T> d = {};
+        FfnProduct<T> &d = list[count++] = {};
         d.A[0] = dg; d.A[1] = du; d.B[0] = f.wg; d.B[1] = f.wu; d.C = f.dx; d.N = f.rows; d.M = f.in; d.K = f.hidden; d.terms = 2;
         d.a_rs = f.hidden; d.a_cs = 1; d.b_rs = f.in; d.b_cs = 1;
-        block_mm<T, FFN_PLAIN>(sc, d);
     }
     auto weights = [&](const T *left, const T *right, T *dw, int N, int M) {
         if (!dw) return;
-        FfnProduct<T> d = {};
+        FfnProduct<T> &d = list[count++] = {};
         d.A[0] = left; d.B[0] = right; d.C = dw; d.N = N; d.M = M; d.K = f.rows; d.terms = 1;
         d.a_rs = 1; d.a_cs = N; d.b_rs = M; d.b_cs = 1;
-        block_mm<T, FFN_PLAIN>(sc, d);
     };
     weights(dg, f.x, f.dwg, f.hidden, f.in);
     weights(du, f.x, f.dwu, f.hidden, f.in);
     weights(f.dy, h, f.dwd, f.out, f.hidden);
+    block_mm<T, FFN_PLAIN>(sc, list, count);
 }
 template void gated_ffn_fw<float>(Scope &, const GatedFfn<float> &);
 template void gated_ffn_fw<__half>(Scope &, const GatedFfn<__half> &);

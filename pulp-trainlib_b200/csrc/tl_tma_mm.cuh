@@ -77,12 +77,9 @@ __device__ __forceinline__ void tm_cluster_sync()
 template <class T> struct PackOp { const T *src; T *dst, *lo; long long rs, cs, bs; int rows, K, Kp, nk, nr, first, straight, vec; };
 template <class T> struct PackOps { PackOp<T> op[2]; int count; };
 
-template <class T>
-__global__ void __launch_bounds__(256) pack_kmajor_kernel(const __grid_constant__ PackOps<T> ops)
+template <class T> __device__ __forceinline__ void pack_kmajor_block(const PackOp<T> &o)
 {
-    pdl_wait();
     __shared__ float tile[32][65];
-    const PackOp<T> &o = ops.op[ops.count > 1 && (int)blockIdx.x >= ops.op[1].first ? 1 : 0];
     const int t = (int)blockIdx.x - o.first, tr = t / o.nk, b = tr / o.nr;
     if (!o.straight) {
         const int k0 = (t - tr * o.nk) * 32, r0 = (tr - b * o.nr) * 64, left = o.rows - r0;
@@ -168,6 +165,12 @@ __global__ void __launch_bounds__(256) pack_kmajor_kernel(const __grid_constant_
         for (int q = 0; q < 4; q++) { const __half2 h = __floats2half2_rn(v[2 * q], v[2 * q + 1]); w[q] = *reinterpret_cast<const uint32_t *>(&h); }
         *reinterpret_cast<uint4 *>(o.dst + at) = make_uint4(w[0], w[1], w[2], w[3]);
     }
+}
+template <class T>
+__global__ void __launch_bounds__(256) pack_kmajor_kernel(const __grid_constant__ PackOps<T> ops)
+{
+    pdl_wait();
+    pack_kmajor_block<T>(ops.op[ops.count > 1 && (int)blockIdx.x >= ops.op[1].first ? 1 : 0]);
 }
 
 // inner: extent of the contiguous index, outer: of the other one, `os` elements apart

@@ -376,7 +376,9 @@ def test_ffn_backward(ops, rows, n, h, m, dt):
         ops.ffn_bw(x, None, None, wd, g, u, dy, None, alone[1], None, None, sizes=s)
         ops.ffn_bw(x, None, None, wd, g, u, dy, None, None, alone[2], None, sizes=s)
         ops.ffn_bw(None, None, None, None, g, u, dy, None, None, None, alone[3], sizes=s)
-        assert all(torch.equal(a, b) for a, b in zip(alone, got))
+        # (a launch of all of them may share a sum's terms out differently: the same bounds, not the same bits)
+        for t, v, q, k, what in zip(alone, want, terms, (2 * h, rows, rows, rows), ("dx", "dw_gate", "dw_up", "dw_down")):
+            near(t, v, dt, 2, (m, k), what + " alone", q)
 
 
 @both
