@@ -381,6 +381,31 @@ def test_ffn_backward(ops, rows, n, h, m, dt):
             near(t, v, dt, 2, (m, k), what + " alone", q)
 
 
+@pytest.mark.parametrize("rows,n,h,m", [(4100, 136, 8200, 2048), (4096, 2048, 2056, 1000), (2300, 1032, 8192, 264), (4100, 136, 8199, 2050)])
+def test_ffn_of_many_tiles(ops, rows, n, h, m):
+    """sizes whose products run on pairs of CTAs, some with rows and columns behind the last whole tile, some that are not read in place"""
+    dt = torch.float16
+    x, wg, wu, wd = ffn_tensors(rows, n, h, m, dt)
+    gd, ud = x.double() @ wg.double().T, x.double() @ wu.double().T
+    want, terms = (silu(gd) * ud) @ wd.double().T, (silu(gd) * ud).square() @ wd.double().square().T
+    y, g, u = blank(rows, m, dt=dt), blank(rows, h, dt=dt), blank(rows, h, dt=dt)
+    ops.ffn_fw(x, wg, wu, wd, g, u, y)
+    near(y, want, dt, 2, (3 * n, h), "y", terms)
+    near(g, gd, dt, 1, (n,), "gate")
+    near(u, ud, dt, 1, (n,), "up")
+    dy = randn(42, rows, m, dt=dt)
+    want, terms = ffn_bw_ref(x, wg, wu, wd, g, u, dy)
+    room = [torch.full((t.numel() + 4096,), 77, device="cuda", dtype=dt) for t in (x, wg, wu, wd)]
+    got = [r[:t.numel()].view_as(t) for r, t in zip(room, (x, wg, wu, wd))]
+    ops.ffn_bw(x, wg, wu, wd, g, u, dy, *got)
+    for t, v, q, k, what in zip(got, want, terms, (2 * h, rows, rows, rows), ("dx", "dw_gate", "dw_up", "dw_down")):
+        near(t, v, dt, 2, (m, k), what, q)
+    assert all((r[t.numel():] == 77).all() for r, t in zip(room, got))
+    again = [blank(*t.shape, dt=dt) for t in got]
+    ops.ffn_bw(x, wg, wu, wd, g, u, dy, *again)
+    assert all(torch.equal(a, b) for a, b in zip(again, got))
+
+
 @both
 def test_ffn_rows_of_no_numbers_stay_apart(ops, dt):
     for rows, n, h, m in ((3, 64, 96, 40), (200, 256, 384, 128), (300, 100, 70, 50)):
