@@ -8,16 +8,18 @@
 //   (Rings in shared memory with even shares of all bytes for persistent CTAs, by bulk copies of 1 KB or by cp.async, keep more under way, but lose more than
 //   that at the ends of the units: 8-bit 4096 -> 10240 for one token 16 us against 11, fp16 4096 x 10240 x 4096 57 us against 54.)
 //   Rows that do not start on 16 bytes come as the five words around the thread's bytes, shifted into place.
-// Single precision: the same on FFMA, a warp's lanes along K, a few rows at a time by up to eight tokens.
+//   Single precision: the same on m16n8k8 in TF32, every operand as two parts and three products of them; the sums move to others, rounded to nearest, after
+//   each turn (the instruction's own sum is cut off towards zero at every step).
 #include "tl_gate.cuh"
+#include "tl_tc.cuh"
 #include "tl_reduce.cuh"
 
 namespace tl {
 
-enum { FEW_F16 = 0, FEW_I8 = 1 };
-static constexpr int FEW_WARPS = 8;                  // of the single-precision kernel
-template <bool I8> struct FewType { typedef __half E; typedef float S; };
-template <> struct FewType<true> { typedef signed char E; typedef int S; };
+enum { FEW_F16 = 0, FEW_I8 = 1, FEW_F32 = 2 };
+template <int KIND> struct FewType { typedef __half E; typedef float S; };
+template <> struct FewType<FEW_I8> { typedef signed char E; typedef int S; };
+template <> struct FewType<FEW_F32> { typedef float E; typedef float S; };
 
 template <class T> struct FewParams {
     const void *x, *w[2];
@@ -44,8 +46,8 @@ template <class E, int ALIGN> __device__ __forceinline__ uint4 few_load(const E 
 #pragma unroll
         for (int i = 0; i < N; i++) {
             uint32_t e = 0;
-            if (k + i < K) { if constexpr (sizeof(E) == 2) e = *reinterpret_cast<const unsigned short *>(row + k + i); else e = *reinterpret_cast<const unsigned char *>(row + k + i); }
-            w[i * 4 / N] |= e << (i % (N / 4) * 8 * (int)sizeof(E));
+            if (k + i < K) { if constexpr (sizeof(E) == 4) e = *reinterpret_cast<const uint32_t *>(row + k + i); else if constexpr (sizeof(E) == 2) e = *reinterpret_cast<const unsigned short *>(row + k + i); else e = *reinterpret_cast<const unsigned char *>(row + k + i); }
+            if constexpr (sizeof(E) == 4) w[i] = e; else w[i * 4 / N] |= e << (i % (N / 4) * 8 * (int)sizeof(E));
         }
         v = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -74,6 +76,16 @@ __device__ __forceinline__ void few_mma(int (&d)[4], uint32_t a0, uint32_t a1, u
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void few_mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void few_split(uint4 v, uint4 &hi, uint4 &lo)
+{
+    tc::split_tf32_rn(__uint_as_float(v.x), hi.x, lo.x); tc::split_tf32_rn(__uint_as_float(v.y), hi.y, lo.y);
+    tc::split_tf32_rn(__uint_as_float(v.z), hi.z, lo.z); tc::split_tf32_rn(__uint_as_float(v.w), hi.w, lo.w);
+}
 // a result: v (and w, the second matrix') of token n and weight row m
 template <class T, int EPI, class S> __device__ __forceinline__ void few_result(const FewParams<T> &p, int n, int m, S v, S w)
 {
@@ -90,11 +102,12 @@ template <int KIND, class T, int EPI, int NT, int MT, int ALIGN, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const __grid_constant__ FewParams<T> p)
 {
     pdl_wait();
-    typedef typename FewType<KIND == FEW_I8>::E E;
-    typedef typename FewType<KIND == FEW_I8>::S S;
+    typedef typename FewType<KIND>::E E;
+    typedef typename FewType<KIND>::S S;
     constexpr int MATS = EPI == FFN_GATE ? 2 : 1, N = 16 / (int)sizeof(E), PIECE = 4 * N;
     // pieces of a turn: 256 bytes of weights per thread, 128 where the tokens take as many registers
-    constexpr int U = (NT > 1 ? 4 : 8) / (MATS * MT);
+    constexpr bool F32 = KIND == FEW_F32;
+    constexpr int U = (NT > 1 || F32 ? 4 : 8) / (MATS * MT);
     __shared__ S red[WARPS][MATS * MT * NT * 4][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, m0 = blockIdx.x * 16 * MT;
     const E *x = reinterpret_cast<const E *>(p.x);
@@ -112,16 +125,49 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
 #pragma unroll
     for (int n = 0; n < NT; n++) xp[n] = x + min(8 * n + g, p.rows - 1) * p.x_stride;
     auto multiply = [&](const uint4 (&wv)[MATS][MT][2], const uint4 (&xv)[NT]) {
+        if constexpr (F32) {
+            uint4 xh[NT], xl[NT];
 #pragma unroll
-        for (int b = 0; b < MATS; b++)
+            for (int n = 0; n < NT; n++) few_split(xv[n], xh[n], xl[n]);
 #pragma unroll
-            for (int a = 0; a < MT; a++)
+            for (int b = 0; b < MATS; b++)
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const uint4 lo = wv[b][a][0], hi = wv[b][a][1], y = xv[n];
-                    few_mma(acc[b][a][n], lo.x, hi.x, lo.y, hi.y, y.x, y.y);
-                    few_mma(acc[b][a][n], lo.z, hi.z, lo.w, hi.w, y.z, y.w);
+                for (int a = 0; a < MT; a++) {
+                    uint4 ph, pl, qh, ql;
+                    few_split(wv[b][a][0], ph, pl);
+                    few_split(wv[b][a][1], qh, ql);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        few_mma_tf32(acc[b][a][n], pl.x, ql.x, pl.y, ql.y, xh[n].x, xh[n].y);
+                        few_mma_tf32(acc[b][a][n], pl.z, ql.z, pl.w, ql.w, xh[n].z, xh[n].w);
+                        few_mma_tf32(acc[b][a][n], ph.x, qh.x, ph.y, qh.y, xl[n].x, xl[n].y);
+                        few_mma_tf32(acc[b][a][n], ph.z, qh.z, ph.w, qh.w, xl[n].z, xl[n].w);
+                        few_mma_tf32(acc[b][a][n], ph.x, qh.x, ph.y, qh.y, xh[n].x, xh[n].y);
+                        few_mma_tf32(acc[b][a][n], ph.z, qh.z, ph.w, qh.w, xh[n].z, xh[n].w);
+                    }
                 }
+        } else {
+#pragma unroll
+            for (int b = 0; b < MATS; b++)
+#pragma unroll
+                for (int a = 0; a < MT; a++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint4 lo = wv[b][a][0], hi = wv[b][a][1], y = xv[n];
+                        few_mma(acc[b][a][n], lo.x, hi.x, lo.y, hi.y, y.x, y.y);
+                        few_mma(acc[b][a][n], lo.z, hi.z, lo.w, hi.w, y.z, y.w);
+                    }
+        }
+    };
+    constexpr int ACCS = MATS * MT * NT * 4;
+    float total[F32 ? ACCS : 1];
+#pragma unroll
+    for (int a = 0; a < (F32 ? ACCS : 1); a++) total[a] = 0.f;
+    auto settle = [&]() {
+        if constexpr (F32) {
+#pragma unroll
+            for (int a = 0; a < ACCS; a++) { total[a] += (&acc[0][0][0][0])[a]; (&acc[0][0][0][0])[a] = 0.f; }
+        }
     };
     int k0 = 0;
     if constexpr (ALIGN == 16) {
@@ -143,6 +189,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
                 for (int n = 0; n < NT; n++) xv[i][n] = few_keep(xp[n] + k0 + (i * WARPS + warp) * PIECE + t * N);
 #pragma unroll
             for (int i = 0; i < U; i++) multiply(wv[i], xv[i]);
+            settle();
         }
     }
     constexpr int UT = ALIGN == 16 ? 1 : MT * MATS == 1 ? 4 : 2;
@@ -162,9 +209,10 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
         }
 #pragma unroll
         for (int i = 0; i < UT; i++) multiply(wv[i], xv[i]);
+        settle();
     }
 #pragma unroll
-    for (int a = 0; a < MATS * MT * NT * 4; a++) red[warp][a][lane] = (&acc[0][0][0][0])[a];
+    for (int a = 0; a < MATS * MT * NT * 4; a++) { if constexpr (F32) red[warp][a][lane] = total[a]; else red[warp][a][lane] = (&acc[0][0][0][0])[a]; }
     __syncthreads();
     // accumulator c of lane (g, t): weight row g + 8 (c / 2), token 2 t + c % 2
     for (int e = threadIdx.x; e < MT * 16 * NT * 8; e += 32 * WARPS) {
@@ -181,20 +229,21 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
     }
 }
 
-// Single precision: R rows of each matrix per CTA, its warps share K, lanes along it; NT tokens (blockIdx.y: which).  V: elements per load.
+// Single precision, up to four tokens, on FFMA: R rows of each matrix per CTA, its warps share K, lanes along it.  V: elements per load.  (One token, 1024 x 2048 x
+// 1024: 6.4 us, on the tensor cores 9.8; rows of odd length 7.9 and 21.6.  Eight tokens: 20.7 and 10.2.)
 template <int EPI, int NT, int R, int V>
-__global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_fp32_kernel(const __grid_constant__ FewParams<float> p)
+__global__ void __launch_bounds__(256) few_rows_fp32_kernel(const __grid_constant__ FewParams<float> p)
 {
     pdl_wait();
     constexpr int MATS = EPI == FFN_GATE ? 2 : 1;
-    __shared__ float red[FEW_WARPS][MATS * R * NT];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = blockIdx.x * R, n0 = blockIdx.y * NT;
+    __shared__ float red[8][MATS * R * NT];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = blockIdx.x * R;
     const float *x = reinterpret_cast<const float *>(p.x);
     float acc[MATS][R][NT];
 #pragma unroll
     for (int a = 0; a < MATS * R * NT; a++) (&acc[0][0][0])[a] = 0.f;
 #pragma unroll 2
-    for (int k = threadIdx.x * V; k < p.K; k += 32 * FEW_WARPS * V) {
+    for (int k = threadIdx.x * V; k < p.K; k += 256 * V) {
         float wv[MATS][R][V], xv[NT][V];
         auto load = [&](const float *row, bool live, float (&v)[V]) {
             if constexpr (V == 4) {
@@ -207,7 +256,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_fp32_kernel(const __g
 #pragma unroll
             for (int r = 0; r < R; r++) load(reinterpret_cast<const float *>(p.w[b]) + (long long)(m0 + r) * p.K, m0 + r < p.M, wv[b][r]);
 #pragma unroll
-        for (int n = 0; n < NT; n++) load(x + (n0 + n) * p.x_stride, n0 + n < p.rows, xv[n]);
+        for (int n = 0; n < NT; n++) load(x + n * p.x_stride, n < p.rows, xv[n]);
 #pragma unroll
         for (int b = 0; b < MATS; b++)
 #pragma unroll
@@ -226,14 +275,14 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_fp32_kernel(const __g
     const int e = threadIdx.x;
     if (e >= R * NT) return;
     const int r = e % R, n = e / R;
-    if (n0 + n >= p.rows || m0 + r >= p.M) return;
+    if (n >= p.rows || m0 + r >= p.M) return;
     float v = 0.f, w = 0.f;
 #pragma unroll
-    for (int k = 0; k < FEW_WARPS; k++) {
+    for (int k = 0; k < 8; k++) {
         v += red[k][r * NT + n];
         if constexpr (MATS == 2) w += red[k][(R + r) * NT + n];
     }
-    few_result<float, EPI, float>(p, n0 + n, m0 + r, v, w);
+    few_result<float, EPI, float>(p, n, m0 + r, v, w);
 }
 
 template <int KIND, class T, int EPI, int NT, int MT, int ALIGN> static void few_launch(const FewParams<T> &p)
@@ -265,9 +314,9 @@ template <int EPI> static void few_fp32(const FewParams<float> &p)
 {
     constexpr int R = EPI == FFN_GATE ? 2 : 4;
     const bool wide = (((uintptr_t)p.x | (uintptr_t)p.w[0] | (uintptr_t)(EPI == FFN_GATE ? p.w[1] : nullptr)) & 15) == 0 && p.K % 4 == 0 && p.x_stride % 4 == 0;
-#define TL_FEW32(NT, V) TL_LAUNCH((few_rows_fp32_kernel<EPI, NT, R, V>), dim3(ceil_div(p.M, R), ceil_div(p.rows, NT)), 32 * FEW_WARPS, 0, p)
-    if (wide) { if (p.rows == 1) TL_FEW32(1, 4); else if (p.rows <= 4) TL_FEW32(4, 4); else TL_FEW32(8, 4); }
-    else { if (p.rows == 1) TL_FEW32(1, 1); else if (p.rows <= 4) TL_FEW32(4, 1); else TL_FEW32(8, 1); }
+#define TL_FEW32(NT, V) TL_LAUNCH((few_rows_fp32_kernel<EPI, NT, R, V>), ceil_div(p.M, R), 256, 0, p)
+    if (wide) { if (p.rows == 1) TL_FEW32(1, 4); else TL_FEW32(4, 4); }
+    else { if (p.rows == 1) TL_FEW32(1, 1); else TL_FEW32(4, 1); }
 #undef TL_FEW32
 }
 
@@ -276,7 +325,8 @@ template <class T, int EPI> void few_rows_mm(Scope &, const FfnProduct<T> &f, lo
     FewParams<T> p = {};
     p.x = f.A[0]; p.w[0] = f.B[0]; p.w[1] = f.B[1]; p.C = f.C; p.g = f.g; p.u = f.u; p.rows = f.N; p.M = f.M; p.K = f.K; p.x_stride = f.a_rs; p.c_stride = c_stride;
     if constexpr (sizeof(T) == 2) few_aligned<FEW_F16, T, EPI>(p, 2);
-    else few_fp32<EPI>(p);
+    else if (p.rows <= 4) few_fp32<EPI>(p);
+    else few_aligned<FEW_F32, T, EPI>(p, 4);
 }
 template <class T> void few_rows_int8(Scope &, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out)
 {
