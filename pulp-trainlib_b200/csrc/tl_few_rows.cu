@@ -8,6 +8,8 @@
 //   (Rings in shared memory with even shares of all bytes for persistent CTAs, by bulk copies of 1 KB or by cp.async, keep more under way, but lose more than
 //   that at the ends of the units: 8-bit 4096 -> 10240 for one token 16 us against 11, fp16 4096 x 10240 x 4096 57 us against 54.)
 //   Rows that do not start on 16 bytes come as the five words around the thread's bytes, shifted into place.
+//   Half precision, up to eight tokens: silu(gate) * up goes from one product to the other in two halves, itself and what its rounding left: the weights' bytes
+//   are what counts, and the result is rounded once (one token of 4096 x 10240 x 4096: 45.9 us, with one rounded half 44.4; 32 tokens would take 76 for 66).
 //   Single precision: the same on m16n8k8 in TF32, every operand as two parts and three products of them; the sums move to others, rounded to nearest, after
 //   each turn (the instruction's own sum is cut off towards zero at every step).
 #include "tl_gate.cuh"
@@ -22,8 +24,8 @@ template <> struct FewType<FEW_I8> { typedef signed char E; typedef int S; };
 template <> struct FewType<FEW_F32> { typedef float E; typedef float S; };
 
 template <class T> struct FewParams {
-    const void *x, *w[2];
-    T *C, *g, *u;
+    const void *x, *x2, *w[2];          // x2: what rounding x to its type left (FFN_PLAIN in half precision)
+    T *C, *C2, *g, *u;                  // C2: what rounding C left (FFN_GATE in half precision)
     const T *bias; const float *xs, *ws;
     int rows, M, K;                     // tokens, weight rows, elements of K
     long long x_stride, c_stride;       // elements
@@ -92,7 +94,9 @@ template <class T, int EPI, class S> __device__ __forceinline__ void few_result(
     const long long at = n * p.c_stride + m;
     if constexpr (EPI == FFN_GATE) {
         if (p.g) { st(p.g + (long long)n * p.M + m, v); st(p.u + (long long)n * p.M + m, w); }
-        st(p.C + at, gate_fw<sizeof(T) == 2>(v, w));
+        const float h = gate_fw<sizeof(T) == 2>(v, w);
+        st(p.C + at, h);
+        if constexpr (sizeof(T) == 2) if (p.C2) { const float rest = h - ld(p.C + at); st(p.C2 + at, fabsf(rest) < INFINITY ? rest : 0.f); }      // (nothing is left of an infinity)
     } else if constexpr (EPI == FFN_INT8) st(p.C + at, (float)v * p.xs[n] * p.ws[m] + ld0(p.bias != nullptr, p.bias + m));
     else st(p.C + at, v);
 }
@@ -106,8 +110,8 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
     typedef typename FewType<KIND>::S S;
     constexpr int MATS = EPI == FFN_GATE ? 2 : 1, N = 16 / (int)sizeof(E), PIECE = 4 * N;
     // pieces of a turn: 256 bytes of weights per thread, 128 where the tokens take as many registers
-    constexpr bool F32 = KIND == FEW_F32;
-    constexpr int U = (NT > 1 || F32 ? 4 : 8) / (MATS * MT);
+    constexpr bool F32 = KIND == FEW_F32, TWO = KIND == FEW_F16 && EPI == FFN_PLAIN && NT == 1;      // TWO: the tokens in two parts
+    constexpr int U = (NT > 1 || F32 || TWO ? 4 : 8) / (MATS * MT);
     __shared__ S red[WARPS][MATS * MT * NT * 4][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, m0 = blockIdx.x * 16 * MT;
     const E *x = reinterpret_cast<const E *>(p.x);
@@ -116,6 +120,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
     for (int a = 0; a < MATS * MT * NT * 4; a++) (&acc[0][0][0][0])[a] = 0;
     // rows behind the last are the last once more (their results are not written): no load has a condition
     const E *wp[MATS][MT][2], *xp[NT];
+    const long long rest = TWO ? reinterpret_cast<const E *>(p.x2) - x : 0;
 #pragma unroll
     for (int b = 0; b < MATS; b++)
 #pragma unroll
@@ -124,7 +129,8 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
             for (int h = 0; h < 2; h++) wp[b][a][h] = reinterpret_cast<const E *>(p.w[b]) + (long long)min(m0 + 16 * a + g + 8 * h, p.M - 1) * p.K;
 #pragma unroll
     for (int n = 0; n < NT; n++) xp[n] = x + min(8 * n + g, p.rows - 1) * p.x_stride;
-    auto multiply = [&](const uint4 (&wv)[MATS][MT][2], const uint4 (&xv)[NT]) {
+    constexpr int XP = TWO ? 2 : 1;
+    auto multiply = [&](const uint4 (&wv)[MATS][MT][2], const uint4 (&xv)[XP * NT]) {
         if constexpr (F32) {
             uint4 xh[NT], xl[NT];
 #pragma unroll
@@ -152,10 +158,10 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
 #pragma unroll
                 for (int a = 0; a < MT; a++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
+                    for (int n = 0; n < XP * NT; n++) {
                         const uint4 lo = wv[b][a][0], hi = wv[b][a][1], y = xv[n];
-                        few_mma(acc[b][a][n], lo.x, hi.x, lo.y, hi.y, y.x, y.y);
-                        few_mma(acc[b][a][n], lo.z, hi.z, lo.w, hi.w, y.z, y.w);
+                        few_mma(acc[b][a][n % NT], lo.x, hi.x, lo.y, hi.y, y.x, y.y);
+                        few_mma(acc[b][a][n % NT], lo.z, hi.z, lo.w, hi.w, y.z, y.w);
                     }
         }
     };
@@ -172,7 +178,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
     int k0 = 0;
     if constexpr (ALIGN == 16) {
         for (; k0 + WARPS * PIECE * U <= p.K; k0 += WARPS * PIECE * U) {
-            uint4 wv[U][MATS][MT][2], xv[U][NT];
+            uint4 wv[U][MATS][MT][2], xv[U][XP * NT];
 #pragma unroll
             for (int i = 0; i < U; i++) {
                 const int k = k0 + (i * WARPS + warp) * PIECE + t * N;
@@ -186,7 +192,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
 #pragma unroll
             for (int i = 0; i < U; i++)
 #pragma unroll
-                for (int n = 0; n < NT; n++) xv[i][n] = few_keep(xp[n] + k0 + (i * WARPS + warp) * PIECE + t * N);
+                for (int n = 0; n < XP * NT; n++) xv[i][n] = few_keep(xp[n % NT] + (n < NT ? 0 : rest) + k0 + (i * WARPS + warp) * PIECE + t * N);
 #pragma unroll
             for (int i = 0; i < U; i++) multiply(wv[i], xv[i]);
             settle();
@@ -194,7 +200,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
     }
     constexpr int UT = ALIGN == 16 ? 1 : MT * MATS == 1 ? 4 : 2;
     for (; k0 < p.K; k0 += WARPS * PIECE * UT) {
-        uint4 wv[UT][MATS][MT][2], xv[UT][NT];
+        uint4 wv[UT][MATS][MT][2], xv[UT][XP * NT];
 #pragma unroll
         for (int i = 0; i < UT; i++) {
             const int k = k0 + (i * WARPS + warp) * PIECE + t * N;
@@ -205,7 +211,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
 #pragma unroll
                     for (int h = 0; h < 2; h++) wv[i][b][a][h] = few_load<E, ALIGN>(wp[b][a][h], k, p.K);
 #pragma unroll
-            for (int n = 0; n < NT; n++) xv[i][n] = few_load<E, ALIGN>(xp[n], k, p.K);
+            for (int n = 0; n < XP * NT; n++) xv[i][n] = few_load<E, ALIGN>(xp[n % NT] + (n < NT ? 0 : rest), k, p.K);
         }
 #pragma unroll
         for (int i = 0; i < UT; i++) multiply(wv[i], xv[i]);
@@ -306,7 +312,7 @@ template <int KIND, class T, int EPI, int ALIGN> static void few_tokens(const Fe
 }
 template <int KIND, class T, int EPI> static void few_aligned(const FewParams<T> &p, int esize)
 {
-    const uintptr_t at = (uintptr_t)p.x | (uintptr_t)p.w[0] | (uintptr_t)(EPI == FFN_GATE ? p.w[1] : nullptr) | (uintptr_t)((long long)p.K * esize) | (uintptr_t)(p.x_stride * esize);
+    const uintptr_t at = (uintptr_t)p.x | (uintptr_t)p.x2 | (uintptr_t)p.w[0] | (uintptr_t)(EPI == FFN_GATE ? p.w[1] : nullptr) | (uintptr_t)((long long)p.K * esize) | (uintptr_t)(p.x_stride * esize);
     if (at % 16 == 0) few_tokens<KIND, T, EPI, 16>(p);
     else few_tokens<KIND, T, EPI, 1>(p);
 }
@@ -320,10 +326,10 @@ template <int EPI> static void few_fp32(const FewParams<float> &p)
 #undef TL_FEW32
 }
 
-template <class T, int EPI> void few_rows_mm(Scope &, const FfnProduct<T> &f, long long c_stride)
+template <class T, int EPI> void few_rows_mm(Scope &, const FfnProduct<T> &f, long long c_stride, const T *x2, T *c2)
 {
     FewParams<T> p = {};
-    p.x = f.A[0]; p.w[0] = f.B[0]; p.w[1] = f.B[1]; p.C = f.C; p.g = f.g; p.u = f.u; p.rows = f.N; p.M = f.M; p.K = f.K; p.x_stride = f.a_rs; p.c_stride = c_stride;
+    p.x = f.A[0]; p.w[0] = f.B[0]; p.w[1] = f.B[1]; p.C = f.C; p.g = f.g; p.u = f.u; p.rows = f.N; p.M = f.M; p.K = f.K; p.x_stride = f.a_rs; p.c_stride = c_stride; p.x2 = x2; p.C2 = c2;
     if constexpr (sizeof(T) == 2) few_aligned<FEW_F16, T, EPI>(p, 2);
     else if (p.rows <= 4) few_fp32<EPI>(p);
     else few_aligned<FEW_F32, T, EPI>(p, 4);
@@ -335,8 +341,8 @@ template <class T> void few_rows_int8(Scope &, const signed char *x, const float
     few_aligned<FEW_I8, T, FFN_INT8>(p, 1);
 }
 #define INST(T)                                                                 \
-    template void few_rows_mm<T, FFN_PLAIN>(Scope &, const FfnProduct<T> &, long long);  \
-    template void few_rows_mm<T, FFN_GATE>(Scope &, const FfnProduct<T> &, long long);   \
+    template void few_rows_mm<T, FFN_PLAIN>(Scope &, const FfnProduct<T> &, long long, const T *, T *);  \
+    template void few_rows_mm<T, FFN_GATE>(Scope &, const FfnProduct<T> &, long long, const T *, T *);   \
     template void few_rows_int8<T>(Scope &, const signed char *, const float *, const signed char *, const float *, const T *, T *, int, int, int);
 INST(float)
 INST(__half)

@@ -33,9 +33,11 @@ template <class T> struct FfnProduct {
 // On the tensor cores (tl_block_mm.cu); false: nothing launched, the error is set (no memory for an operand's copy, no tensor-map encoder)
 // FFN_PLAIN: up to four products in one launch, none of which may write what another one reads.
 template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> *list, int count);
-// Few tokens (FEW_ROWS at most), weights with K contiguous (tl_few_rows.cu): FFN_PLAIN of one term and FFN_GATE.  c_stride: elements between the rows of C.
-static constexpr int FEW_ROWS = 32;
-template <class T, int EPI> void few_rows_mm(Scope &sc, const FfnProduct<T> &p, long long c_stride);
+// Few tokens (FEW_ROWS at most), weights with K contiguous (tl_few_rows.cu): FFN_PLAIN of one term and FFN_GATE.  c_stride: elements between the
+// rows of C.  Half precision, FEW_TWO tokens at most: FFN_GATE leaves what rounding C left in c2, FFN_PLAIN adds the product of x2 with the
+// same weights.
+static constexpr int FEW_ROWS = 32, FEW_TWO = 8;
+template <class T, int EPI> void few_rows_mm(Scope &sc, const FfnProduct<T> &p, long long c_stride, const T *x2, T *c2);
 template <class T> void few_rows_int8(Scope &sc, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out);
 
 } // namespace tl

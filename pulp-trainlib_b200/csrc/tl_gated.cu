@@ -18,20 +18,20 @@ template <class T> __global__ void __launch_bounds__(256) gate_kernel(const T *_
 
 template <class T> void gated_ffn_fw(Scope &sc, const GatedFfn<T> &f)
 {
-    // few tokens: H in rows of whole 16-byte pieces
-    const bool few = f.rows <= FEW_ROWS;
+    // few tokens: H in rows of whole 16-byte pieces, in half precision with what its rounding left beside it
+    const bool few = f.rows <= FEW_ROWS, two = sizeof(T) == 2 && f.rows <= FEW_TWO;
     const int pitch = few ? (f.hidden + 7) / 8 * 8 : f.hidden;
-    T *h = sc.scratch<T>((size_t)f.rows * pitch);
-    if (!h) return;
+    T *h = sc.scratch<T>((size_t)f.rows * pitch), *rest = two ? sc.scratch<T>((size_t)f.rows * pitch) : nullptr;
+    if (!h || (two && !rest)) return;
     FfnProduct<T> p = {};
     p.A[0] = f.x; p.B[0] = f.wg; p.B[1] = f.wu; p.C = h; p.g = f.g; p.u = f.u; p.N = f.rows; p.M = f.hidden; p.K = f.in; p.terms = 1;
     p.a_rs = f.in; p.a_cs = 1; p.b_rs = 1; p.b_cs = f.in;
-    if (few) few_rows_mm<T, FFN_GATE>(sc, p, pitch);
+    if (few) few_rows_mm<T, FFN_GATE>(sc, p, pitch, nullptr, rest);
     else if (!block_mm<T, FFN_GATE>(sc, &p, 1)) return;
     FfnProduct<T> d = {};
     d.A[0] = h; d.B[0] = f.wd; d.C = f.y; d.N = f.rows; d.M = f.out; d.K = f.hidden; d.terms = 1;
     d.a_rs = pitch; d.a_cs = 1; d.b_rs = 1; d.b_cs = f.hidden;
-    if (few) few_rows_mm<T, FFN_PLAIN>(sc, d, f.out);
+    if (few) few_rows_mm<T, FFN_PLAIN>(sc, d, f.out, rest, nullptr);
     else block_mm<T, FFN_PLAIN>(sc, &d, 1);
 }
 template <class T> void gated_ffn_bw(Scope &sc, const GatedFfn<T> &f)
