@@ -613,7 +613,9 @@ template <class T, int JOBS> static BmPlan bm_plan(int kind, int epi, BmParams<T
             const double work = p.jobs == 1 ? ceil_div(units, places) * longest : std::max(sum / places + 0.3 * longest, longest);
             const double cost = (two ? 10000.0 : 2000.0) + work + reduce;
             if (cost < 0.97 * best) { best = cost; plan = {bn, two ? 1 : 0}; for (int k = 0; k < p.jobs; k++) p.job[k].splits = splits[k]; }
-            if (two || splits[at] >= 16 || units + tiles[at] > places || p.job[at].ksteps < 2 * (splits[at] + 1)) break;
+            // alone, a product's parts have to fit the CTAs once; among others, parts shorten the unit that the launch would wait for
+            const bool more = p.jobs == 1 ? units + tiles[at] <= places : longest > 0.5 * sum / places && (long long)tiles[at] * (splits[at] + 1) * BM_ROWS * bn <= (16ll << 20);
+            if (two || splits[at] >= 32 || !more || p.job[at].ksteps < 2 * (splits[at] + 1)) break;
             splits[at]++;
             units += tiles[at];
         }
