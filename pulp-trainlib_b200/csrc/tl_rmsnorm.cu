@@ -3,7 +3,8 @@
 //   q = rint(w h * 127 / max|w h|),  scale = r max|w h| / 127        (r > 0 leaves the rounding: it only scales the row)
 //   dx = dsum + r (g - h r^2 mean(g h)),  g = w dy;   dw = sum over the rows of dy h r
 // All of it is bound by its tensors' bytes: a row is read once into registers, by a warp or by a CTA, and everything that depends on it leaves
-// from there.  Rows that no CTA's registers hold (above 32768 elements forward, 16384 backward) are read twice.
+// from there.  Rows that no CTA's registers hold are read twice: forward above 4096 packs of 16 bytes (32768 halves, 16384 floats; of rows that do not start
+// on 16 bytes, 4096 single elements or pairs of halves), backward above 16384 elements.
 #include "tl_kernels.h"
 #include "tl_reduce.cuh"
 #include "tl_tc.cuh"
@@ -75,7 +76,8 @@ template <class T, int V> __device__ __forceinline__ Pack<T, V> zerov()
 }
 
 // Pairs of single-precision values: one instruction for two products or sums, rounded as two.  What bounds these kernels beside the bytes is the number of
-// instructions per element (31 of them, one by one and with every load under a condition of its own, held the half-precision backward pass at 4 TB/s).
+// instructions per element: 31 of them, one by one and with every load under a condition of its own, held the half-precision backward pass at 4 TB/s, and the
+// half-precision forward pass at 8192 columns took 57 us value by value, 41 us in pairs.
 __device__ __forceinline__ uint64_t pair_bits(float2 v) { return *reinterpret_cast<const uint64_t *>(&v); }
 __device__ __forceinline__ float2 pair(uint64_t v) { return *reinterpret_cast<const float2 *>(&v); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
@@ -179,33 +181,40 @@ __device__ __forceinline__ void norm_leave(float (&h)[V], const Pack<T, V> &wv, 
         stv<signed char, V>(q + at, o);
     }
 }
-// dw's partial sum of a block from its RG groups of rows, one behind the other
+// dw's partial sum of a block from its RG groups of rows, the groups in order; cols: [RG, size]
 template <class T, int G, int NV, int V, int RG, int TPB>
 __device__ __forceinline__ void block_columns(const float (&acc)[NV][V], float *out, float *cols, int size, int t, int mine)
 {
-    if constexpr (RG == 1) {
+    if constexpr (RG > 1) __syncthreads();                   // (the ring's memory is read no more)
+    float *to = RG > 1 ? cols + mine * size : out;
 #pragma unroll
-        for (int k = 0; k < NV; k++)
+    for (int k = 0; k < NV; k++) {
+        const int j = (k * G + t) * V;
+        constexpr int U = V < 4 ? V : 4;
+        if (j >= size) continue;
 #pragma unroll
-            for (int i = 0; i < V; i++) { const int j = (k * G + t) * V + i; if (j < size) out[j] = acc[k][i]; }
-    } else {
-        for (int g = 0; g < RG; g++) {
-            __syncthreads();
-            if (mine != g) continue;
+        for (int i = 0; i < V; i += U) {
+            Pack<float, U> o;
 #pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int i = 0; i < V; i++) { const int j = (k * G + t) * V + i; if (j < size) cols[j] = g ? cols[j] + acc[k][i] : acc[k][i]; }
+            for (int e = 0; e < U; e++) o.e[e] = acc[k][i + e];
+            stv<float, U>(to + j + i, o);
         }
+    }
+    if constexpr (RG > 1) {
         __syncthreads();
-        for (int j = threadIdx.x; j < size; j += TPB) out[j] = cols[j];
+        for (int j = threadIdx.x; j < size; j += TPB) {
+            float v = cols[j];
+#pragma unroll
+            for (int g = 1; g < RG; g++) v += cols[g * size + j];
+            out[j] = v;
+        }
     }
 }
 
 // ---------------------------------------------------------------- rows through a ring in shared memory
-// Many rows: one CTA per SM whose groups of G threads walk rows of their own.  A group's rows arrive by bulk copies in a ring of stages (IN tensors' rows each),
-// some 200 KB under way per SM whatever the registers hold; a group waits for nobody but its own G threads.  A stage is fetched anew as soon as the
-// group's sums have met: by then all of it is in registers.
+// The backward pass holds its columns' sums of dy h r in registers from row to row, so one CTA per SM walks many rows, and what its registers leave free does not
+// cover the memory's latency.  So the rows arrive by bulk copies in a ring of stages (IN tensors' rows each), some 200 KB under way per SM; a group of G threads
+// walks rows of its own and waits for nobody but itself.  A stage is fetched anew as soon as the group's sums have met: by then all of it is in registers.
 static constexpr int RING_TPB = 512, RING_BYTES = 200 * 1024, RING_MOST = 8;
 template <int G> __device__ __forceinline__ void group_sync()
 {
@@ -300,90 +309,6 @@ template <int V, bool SCALED> __device__ __forceinline__ Pack<signed char, V> qu
     return q;
 }
 
-template <class T, int MODE, int G, int NV, int V>
-__global__ void __launch_bounds__(RING_TPB) rmsnorm_fw_ring_kernel(const T *x, const T *res, const T *__restrict__ w, T *sum, T *y, signed char *__restrict__ q,
-                                                                   float *__restrict__ scale, int rows, int size, int stages, float eps, int *status)
-{
-    pdl_wait();
-    const float per = 1.f / (float)size;
-    constexpr int IN = MODE == QUANT_ROWS ? 1 : 2, P = V / 2;
-    constexpr bool HALVES = MODE == QUANT_ROWS && sizeof(T) == 2;
-    extern __shared__ __align__(128) unsigned char ring_mem[];
-    __shared__ uint64_t full[RING_TPB / G][RING_MOST];
-    __shared__ float2 red[2][RING_TPB / 32];
-    __shared__ int failed;
-    Ring<T, G, IN> ring = make_ring<T, G, IN>(ring_mem, full, &failed, status, stages, size, rows);
-    ring.src[0] = x;
-    if constexpr (IN > 1) ring.src[1] = res;
-    const int t = threadIdx.x % G;
-    ring.start(t);
-    Pack<T, V> wv[NV];
-#pragma unroll
-    for (int k = 0; k < NV; k++) { const int j = (k * G + t) * V; wv[k] = MODE != QUANT_ROWS && j < size ? ldv<T, V>(w + j) : zerov<T, V>(); }
-    int s_at = 0;
-    for (int i = 0; i < ring.count; i++, s_at = s_at + 1 == stages ? 0 : s_at + 1) {
-        const int row = ring.row0 + i * ring.step;
-        const size_t at = (size_t)row * size;
-        ring.wait(i);
-        const T *in0 = ring.stage(s_at, 0), *in1 = ring.stage(s_at, IN - 1);
-        float2 h[NV][P], s2 = twice(0.f);
-        float m = 0.f;
-        Pack<T, V> raw[NV];
-        if constexpr (HALVES) {                              // largest magnitude as it lies, two halves at a time; NaN stays
-            __half2 m2 = __float2half2_rn(0.f);
-#pragma unroll
-            for (int k = 0; k < NV; k++) {
-                const int j = (k * G + t) * V;
-                if (j >= size) continue;
-                raw[k] = ldv<T, V>(in0 + j);
-#pragma unroll
-                for (int e = 0; e < P; e++) m2 = __hmax2_nan(m2, __habs2(*reinterpret_cast<const __half2 *>(&raw[k].e[2 * e])));
-            }
-            m = __half2float(__hmax_nan(__low2half(m2), __high2half(m2)));
-            s2 = twice(m * 0.f);
-        } else
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int j = (k * G + t) * V;
-            if (j >= size) continue;
-            unpack<V>(ldv<T, V>(in0 + j), h[k]);
-            if (IN > 1 && res) {
-                float2 b[P];
-                unpack<V>(ldv<T, V>(in1 + j), b);
-#pragma unroll
-                for (int e = 0; e < P; e++) h[k][e] = add2(h[k][e], b[e]);
-            }
-            float2 ww[P];
-            if (MODE == NORM_INT8) unpack<V>(wv[k], ww);
-#pragma unroll
-            for (int e = 0; e < P; e++) {
-                s2 = fma2(h[k][e], MODE == QUANT_ROWS ? twice(0.f) : h[k][e], s2);       // (quantised alone, the sum tells only whether every value is finite)
-                if (MODE != NORM_PLAIN) { const float2 v = MODE == NORM_INT8 ? mul2(h[k][e], ww[e]) : h[k][e]; m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))); }
-            }
-        }
-        const float2 tot = group_reduce<G, true>(s2.x + s2.y, m, red[i & 1]);
-        ring.refill(i, t);
-        const float r = MODE == QUANT_ROWS ? 1.f : norm_factor(fmaf(tot.x, per, eps));
-        const float2 f = MODE == NORM_PLAIN ? make_float2(0.f, 0.f) : quant_factor(tot.y);
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int j = (k * G + t) * V;
-            if (j >= size) continue;
-            if (MODE != QUANT_ROWS && sum) stv<T, V>(sum + at + j, repack<V>(h[k], (T *)nullptr));
-            if (MODE != QUANT_ROWS) {
-                float2 ww[P];
-                unpack<V>(wv[k], ww);
-#pragma unroll
-                for (int e = 0; e < P; e++) h[k][e] = mul2(MODE == NORM_PLAIN ? mul2(h[k][e], twice(r)) : h[k][e], ww[e]);
-            }
-            if constexpr (HALVES) unpack<V>(raw[k], h[k]);
-            if constexpr (MODE == NORM_PLAIN) stv<T, V>(y + at + j, repack<V>(h[k], (T *)nullptr));
-            else stv<signed char, V>(q + at + j, quant_pairs<V, sizeof(T) == 4 || MODE == NORM_INT8>(h[k], f, tot.y, tot.x - tot.x == 0.f));
-        }
-        if (MODE != NORM_PLAIN && t == 0) scale[row] = quant_scale(r, tot.y, tot.x);
-    }
-    ring.settle(t);
-}
 // backward: as rmsnorm_bw_kernel, below
 template <class T, int G, int NV, int V>
 __global__ void __launch_bounds__(RING_TPB) rmsnorm_bw_ring_kernel(const T *h, const T *__restrict__ w, const T *dy, const T *dsum, T *dx, float *__restrict__ part,
@@ -466,9 +391,13 @@ template <class T> static int ring_stages(int groups, int in, int size)
 }
 
 // ---------------------------------------------------------------- forward
-// G threads per row, a block's rows side by side, NV packs of V elements per thread.
+// G threads per row, a block's rows side by side, NV packs of V elements per thread; small CTAs, so that one's loads cover the other's stores.  Measured with
+// x, residual, sum and y of 2^25 elements (41 us half, 82 us single at the rate of a plain copy): halves 40.4 us at 256 columns, 40.8 at 1000 and 2048, 41.4 at 8192,
+// 44.8 at 16384; floats 79 us from 256 to 8192 columns, 84 at 16384; 999 columns, element by element, 58 and 80 us.
+// (CTAs per SM that the registers are held down to: 1024 threads with 4 or 8 packs each, 768 of 256 with 8, 1280 with fewer)
+constexpr int fw_blocks(int g, int nv, bool few) { return g < 512 ? nv == 8 ? 3 : nv == 4 ? 4 : 5 : nv == 4 || few ? 2 : 1; }
 template <class T, int MODE, int G, int NV, int V>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) rmsnorm_fw_kernel(const T *x, const T *res, const T *__restrict__ w, T *sum, T *y, signed char *__restrict__ q,
+__global__ void __launch_bounds__(G < 256 ? 256 : G, fw_blocks(G, NV, MODE == QUANT_ROWS || V < 4)) rmsnorm_fw_kernel(const T *x, const T *res, const T *__restrict__ w, T *sum, T *y, signed char *__restrict__ q,
                                                                        float *__restrict__ scale, int rows, int size, float eps)
 {
     pdl_wait();
@@ -486,6 +415,44 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) rmsnorm_fw_kernel(const T *
         if (in) a[k] = ldv<T, V>(x + at + j);
         if (in && res) b[k] = ldv<T, V>(res + at + j);
         if (MODE != QUANT_ROWS && in) wv[k] = ldv<T, V>(w + j);
+    }
+    if constexpr (V >= 4) {
+        constexpr int P = V / 2;
+        float2 h[NV][P], s2 = twice(0.f);
+        float m = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            float2 c[P], ww[P];
+            unpack<V>(a[k], h[k]);
+            unpack<V>(b[k], c);
+            if (MODE == NORM_INT8) unpack<V>(wv[k], ww);
+#pragma unroll
+            for (int e = 0; e < P; e++) {
+                h[k][e] = add2(h[k][e], c[e]);
+                s2 = fma2(h[k][e], MODE == QUANT_ROWS ? twice(0.f) : h[k][e], s2);       // (quantised alone, the sum tells only whether every value is finite)
+                if (MODE != NORM_PLAIN) { const float2 v = MODE == NORM_INT8 ? mul2(h[k][e], ww[e]) : h[k][e]; m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))); }
+            }
+        }
+        const float2 tot = row_reduce<G, true>(s2.x + s2.y, m, red);     // (the largest magnitude passes over NaN: the scale carries it)
+        if (row >= rows) return;
+        const float r = MODE == QUANT_ROWS ? 1.f : norm_factor(fmaf(tot.x, per, eps));
+        const float2 f = MODE == NORM_PLAIN ? make_float2(0.f, 0.f) : quant_factor(tot.y);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int j = (k * G + t) * V;
+            if (j >= size) continue;
+            if (MODE != QUANT_ROWS && sum) stv<T, V>(sum + at + j, repack<V>(h[k], (T *)nullptr));
+            if (MODE != QUANT_ROWS) {
+                float2 ww[P];
+                unpack<V>(wv[k], ww);
+#pragma unroll
+                for (int e = 0; e < P; e++) h[k][e] = mul2(MODE == NORM_PLAIN ? mul2(h[k][e], twice(r)) : h[k][e], ww[e]);
+            }
+            if constexpr (MODE == NORM_PLAIN) stv<T, V>(y + at + j, repack<V>(h[k], (T *)nullptr));
+            else stv<signed char, V>(q + at + j, quant_pairs<V, sizeof(T) == 4 || MODE == NORM_INT8>(h[k], f, tot.y, tot.x - tot.x == 0.f));
+        }
+        if (MODE != NORM_PLAIN && t == 0) scale[row] = quant_scale(r, tot.y, tot.x);
+        return;
     }
     float s = 0.f, m = 0.f, h[NV][V];
 #pragma unroll
@@ -540,6 +507,40 @@ __global__ void __launch_bounds__(1024) rmsnorm_fw_wide_kernel(const T *x, const
     if (MODE != NORM_PLAIN && threadIdx.x == 0) scale[blockIdx.x] = quant_scale(r, tot.y, tot.x);
 }
 
+// The 8-bit form of half-precision rows as they are: a CTA of G threads per row, the halves in registers as they lie, the largest magnitude two at a time.
+// 4096 rows of 8192: 32 us (a ring in shared memory with one CTA per SM: 35), the bytes alone 15; the rounding's fourteen instructions per element hold it there.
+template <int G, int NV>
+__global__ void __launch_bounds__(G, 1280 / G) quantize_rows_kernel(const __half *__restrict__ x, signed char *__restrict__ q, float *__restrict__ scale, int size)
+{
+    pdl_wait();
+    constexpr int V = 8, P = V / 2;
+    __shared__ float2 red[G / 32];
+    const size_t at = (size_t)blockIdx.x * size;
+    Pack<__half, V> raw[NV];
+    __half2 m2 = __float2half2_rn(0.f);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int j = (k * G + threadIdx.x) * V;
+        raw[k] = j < size ? ldv<__half, V>(x + at + j) : zerov<__half, V>();
+    }
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int e = 0; e < P; e++) m2 = __hmax2_nan(m2, __habs2(*reinterpret_cast<const __half2 *>(&raw[k].e[2 * e])));
+    const float m = __half2float(__hmax_nan(__low2half(m2), __high2half(m2)));
+    const float2 tot = row_reduce<G, true>(m * 0.f, m, red);             // the sum tells only whether every value is finite
+    const float2 f = quant_factor(tot.y);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int j = (k * G + threadIdx.x) * V;
+        if (j >= size) continue;
+        float2 h[P];
+        unpack<V>(raw[k], h);
+        stv<signed char, V>(q + at + j, quant_pairs<V, false>(h, f, tot.y, tot.x == 0.f));
+    }
+    if (threadIdx.x == 0) scale[blockIdx.x] = quant_scale(1.f, tot.y, tot.x);
+}
+
 template <class T, int MODE>
 static void norm_forward(const T *x, const T *res, const T *w, T *sum, T *y, signed char *q, float *scale, int rows, int size, float eps)
 {
@@ -547,42 +548,36 @@ static void norm_forward(const T *x, const T *res, const T *w, T *sum, T *y, sig
     // packs of 16 bytes where every row of every tensor starts on such a boundary (the 8-bit one on V16 bytes)
     const uintptr_t at = (uintptr_t)x | (uintptr_t)res | (uintptr_t)w | (uintptr_t)sum | (uintptr_t)y;
     const bool wide = size % V16 == 0 && at % 16 == 0 && (uintptr_t)q % V16 == 0;
-    const int packs = wide ? size / V16 : size;
+    // or of two halves
+    constexpr int V2 = sizeof(T) == 2 ? 2 : 1;
+    const bool two = V2 == 2 && size % 2 == 0 && at % 4 == 0 && (uintptr_t)q % 2 == 0;
+    const int packs = wide ? size / V16 : two ? size / 2 : size;
 #define TL_NORM(G, NV, V) TL_LAUNCH((rmsnorm_fw_kernel<T, MODE, G, NV, V>), ceil_div(rows, (G < 256 ? 256 : G) / G), G < 256 ? 256 : G, 0, x, res, w, sum, y, q, scale, rows, size, eps)
 #define TL_NORM_V(V)                                                                                  \
     do {                                                                                              \
+        constexpr bool FEW = MODE == QUANT_ROWS || V < 4;                                             \
         if (packs <= 32) TL_NORM(32, 1, V);                                                           \
         else if (packs <= 64) TL_NORM(32, 2, V);                                                      \
-        else if (packs <= 128 && rows > 4 * sm_count()) TL_NORM(32, 4, V);                            \
-        else if (packs <= 256) TL_NORM(128, 2, V);                                                    \
-        else if (packs <= 512) TL_NORM(256, 2, V);                                                    \
-        else if (packs <= 1024) TL_NORM(512, 2, V);                                                   \
-        else if (packs <= 2048) TL_NORM(1024, 2, V);                                                  \
-        else TL_NORM(1024, 4, V);                                                                     \
+        else if (packs <= 128) TL_NORM((FEW ? 32 : 64), (FEW ? 4 : 2), V);                            \
+        else if (packs <= 256) TL_NORM((FEW ? 32 : 128), (FEW ? 8 : 2), V);                           \
+        else if (packs <= 512) TL_NORM((FEW ? 64 : 256), (FEW ? 8 : 2), V);                           \
+        else if (packs <= 1024) TL_NORM((FEW ? 128 : 256), (FEW ? 8 : 4), V);                         \
+        else if (packs <= 2048) TL_NORM((FEW ? 256 : 512), (FEW ? 8 : 4), V);                         \
+        else TL_NORM(512, 8, V);                                                                      \
     } while (0)
-    if (wide && rows >= 4 * sm_count() && size <= RING_TPB * 32) {
-        int *status = tc_status_word();
-        constexpr int IN = MODE == QUANT_ROWS ? 1 : 2;
-#define TL_NORM_RING(G, NV)                                                                                                                                       \
-    do {                                                                                                                                                          \
-        const int stages = status ? ring_stages<T>(RING_TPB / G, IN, size) : 0;                                                                                   \
-        if (!stages) break;                                                                                                                                       \
-        static bool set = false;                                                                                                                                  \
-        if (!set) set = cudaFuncSetAttribute(rmsnorm_fw_ring_kernel<T, MODE, G, NV, V16>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES) == cudaSuccess; \
-        TL_LAUNCH((rmsnorm_fw_ring_kernel<T, MODE, G, NV, V16>), sm_count(), RING_TPB, RING_BYTES, x, res, w, sum, y, q, scale, rows, size, stages, eps, status);  \
-        return;                                                                                                                                                   \
-    } while (0)
-        constexpr int E = 32 / V16;
-        if (size <= 32 * 16) TL_NORM_RING(32, E / 2);
-        else if (size <= 32 * 32) TL_NORM_RING(32, E);
-        else if (size <= 64 * 32) TL_NORM_RING(64, E);
-        else if (size <= 128 * 32) TL_NORM_RING(128, E);
-        else if (size <= 256 * 32) TL_NORM_RING(256, E);
-        else TL_NORM_RING(512, E);
-#undef TL_NORM_RING
+    if constexpr (MODE == QUANT_ROWS && sizeof(T) == 2) {
+        if (wide && size > 512 && size <= 16384) {
+            if (size <= 1024) TL_LAUNCH((quantize_rows_kernel<128, 1>), rows, 128, 0, x, q, scale, size);
+            else if (size <= 2048) TL_LAUNCH((quantize_rows_kernel<128, 2>), rows, 128, 0, x, q, scale, size);
+            else if (size <= 4096) TL_LAUNCH((quantize_rows_kernel<128, 4>), rows, 128, 0, x, q, scale, size);
+            else if (size <= 8192) TL_LAUNCH((quantize_rows_kernel<256, 4>), rows, 256, 0, x, q, scale, size);
+            else TL_LAUNCH((quantize_rows_kernel<512, 4>), rows, 512, 0, x, q, scale, size);
+            return;
+        }
     }
     if (packs > 4096) TL_LAUNCH((rmsnorm_fw_wide_kernel<T, MODE>), rows, 1024, 0, x, res, w, sum, y, q, scale, size, eps);
     else if (wide) TL_NORM_V(V16);
+    else if (two) TL_NORM_V(V2);
     else TL_NORM_V(1);
 #undef TL_NORM_V
 #undef TL_NORM
@@ -612,7 +607,7 @@ __global__ void __launch_bounds__(G < NB_TPB ? NB_TPB : G) rmsnorm_bw_kernel(con
     const float per = 1.f / (float)size;
     constexpr int TPB = G < NB_TPB ? NB_TPB : G, RG = TPB / G;
     __shared__ float2 red[2][TPB / 32];
-    extern __shared__ float cols[];                      // [size], where RG > 1
+    extern __shared__ __align__(16) float cols[];        // [RG, size], where RG > 1
     const int t = threadIdx.x % G, mine = threadIdx.x / G;
     Pack<T, V> hv[NV], gv[NV];
     float acc[NV][V];
@@ -758,24 +753,24 @@ template <class T> void rmsnorm_bw(Scope &sc, const T *h, const T *w, const T *d
         if (dx) TL_LAUNCH((rmsnorm_bw_dx_kernel<T>), rows, 1024, 0, h, w, dy, dsum, dx, stats, size);
         return;
     }
-    if (wide && size <= RING_TPB * 16) {
+    if (wide && size <= 512 * 16) {
         int *status = tc_status_word();
-#define TL_NORM_BW_RING(G, NV)                                                                                                                                    \
-    do {                                                                                                                                                          \
-        const int stages = status ? ring_stages<T>(RING_TPB / G, 3, size) : 0, blocks = std::min(ceil_div(rows, RING_TPB / G), sm_count());                       \
-        if (!stages) break;                                                                                                                                       \
-        float *part = dw ? sc.scratch<float>((size_t)blocks * size) : nullptr;                                                                                    \
-        if (dw && !part) return;                                                                                                                                  \
-        static bool set = false;                                                                                                                                  \
-        if (!set) set = cudaFuncSetAttribute(rmsnorm_bw_ring_kernel<T, G, NV, V16>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES) == cudaSuccess;      \
-        TL_LAUNCH((rmsnorm_bw_ring_kernel<T, G, NV, V16>), blocks, RING_TPB, RING_BYTES, h, w, dy, dsum, dx, part, rows, size, stages, eps, status);               \
-        if (dw) norm_columns<T>(part, dw, size, blocks);                                                                                                          \
-        return;                                                                                                                                                   \
+#define TL_NORM_BW_RING(G, NV)                                                                                                                                        \
+    do {                                                                                                                                                              \
+        const int stages = status ? ring_stages<T>(RING_TPB / G, 3, size) : 0, blocks = std::min(ceil_div(rows, RING_TPB / G), sm_count());                           \
+        if (!stages) break;                                                                                                                                           \
+        float *part = dw ? sc.scratch<float>((size_t)blocks * size) : nullptr;                                                                                        \
+        if (dw && !part) return;                                                                                                                                      \
+        static bool set = false;                                                                                                                                      \
+        if (!set) set = cudaFuncSetAttribute(rmsnorm_bw_ring_kernel<T, G, NV, V16>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES) == cudaSuccess;          \
+        TL_LAUNCH((rmsnorm_bw_ring_kernel<T, G, NV, V16>), blocks, RING_TPB, RING_BYTES, h, w, dy, dsum, dx, part, rows, size, stages, eps, status);                  \
+        if (dw) norm_columns<T>(part, dw, size, blocks);                                                                                                              \
+        return;                                                                                                                                                       \
     } while (0)
         constexpr int E = 16 / V16;
         if (size <= 32 * 8) TL_NORM_BW_RING(32, (E + 1) / 2);
         else if (size <= 32 * 16) TL_NORM_BW_RING(32, E);
-        else if (size <= 128 * 8) TL_NORM_BW_RING(128, (E + 1) / 2);
+        else if (size <= 64 * 16) TL_NORM_BW_RING(64, E);
         else if (size <= 128 * 16) TL_NORM_BW_RING(128, E);
         else if (size <= 256 * 16) TL_NORM_BW_RING(256, E);
         else TL_NORM_BW_RING(512, E);
@@ -787,7 +782,7 @@ template <class T> void rmsnorm_bw(Scope &sc, const T *h, const T *w, const T *d
         const int blocks = std::min(ceil_div(rows, RG), (TPB == 1024 ? 1 : 2) * sm_count());                                                                  \
         float *part = dw ? sc.scratch<float>((size_t)blocks * size) : nullptr;                                                                                \
         if (dw && !part) return;                                                                                                                              \
-        TL_LAUNCH((rmsnorm_bw_kernel<T, G, NV, V, PRE>), blocks, TPB, RG > 1 ? size * sizeof(float) : 0, h, w, dy, dsum, dx, part, rows, size, eps);          \
+        TL_LAUNCH((rmsnorm_bw_kernel<T, G, NV, V, PRE>), blocks, TPB, RG > 1 ? RG * size * sizeof(float) : 0, h, w, dy, dsum, dx, part, rows, size, eps);          \
         if (dw) norm_columns<T>(part, dw, size, blocks);                                                                                                      \
     } while (0)
 #define TL_NORM_BW_V(V, E)                                                     \
