@@ -29,13 +29,16 @@ template <class T> struct BmJob {
     T *C, *g, *u, *dg, *du;
     const T *bias; const float *xs, *ws;
     uint32_t *part;
-    int N, M, tiles_m, tiles_n, kps, ksteps, splits, first, a_mn, b_mn, vec;               // kps: K steps of a term
+    int N, M, ld, tiles_m, tiles_n, kps, ksteps, splits, first, reduce_first, a_mn, b_mn;  // ld: elements between the rows of C, dg and du (g and u: M); kps: K steps of a term
+    int c_align, g_align;                                                                  // ALIGN_* of C, dg, du and of g, u
 };
+// What all rows of a tensor start on: 16 bytes (and are whole groups of 16 long, or padded so), 4 bytes, or their elements' size
+enum { ALIGN_ELEMENT = 0, ALIGN_WORD = 1, ALIGN_16 = 2 };
 static constexpr int BM_JOBS = 4;
 constexpr int bm_jobs(int epi) { return epi == FFN_PLAIN ? BM_JOBS : 1; }
 template <class T, int JOBS> struct BmParams {
     BmJob<T> job[JOBS];
-    int jobs, units, stages;
+    int jobs, units, stages, reduce_blocks;
     uint32_t stage_bytes;
     int *status;
 };
@@ -126,47 +129,76 @@ template <class T, int W> struct BmTile {
         if constexpr (sizeof(T) == 2) return make_uint4(bm_half2(v[0], v[1]), bm_half2(v[2], v[3]), bm_half2(v[4], v[5]), bm_half2(v[6], v[7]));
         else return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     }
+    // Rows that do not start on 16 bytes move in 32-bit words, neighbouring lanes neighbouring words of a row: in memory as a word where rows start on four bytes,
+    // as two halves otherwise.  (Element by element, each load waited for the one before: with 1650 columns the gradient's epilogue took 38 us, now 10.)
+    static constexpr int WORDS = CHUNKS * 4, ROW_WORDS = W * (int)sizeof(T) / 4;           // of a lane; of a row
+    static __device__ __forceinline__ uint32_t &word(uint4 (&q)[CHUNKS], int i) { return reinterpret_cast<uint32_t *>(&q[i / 4])[i % 4]; }
     // registers -> memory; base: the tensor's element (first row of the warp, first column of the tile); rows, cols: how many of them exist
-    static __device__ __forceinline__ void store(T *base, int M, int rows, int cols, bool vec, const float (&v)[W], unsigned char *stage, int lane)
+    static __device__ __forceinline__ void store(T *base, int ld, int rows, int cols, int align, const float (&v)[W], unsigned char *stage, int lane)
     {
 #pragma unroll
         for (int c = 0; c < CHUNKS; c++) *reinterpret_cast<uint4 *>(stage + at(lane, c)) = pack(v + c * E);
         __syncwarp();
-        if (vec && cols >= W) {
+        if (align == ALIGN_16) {
 #pragma unroll
             for (int i = 0; i < CHUNKS; i++) {
                 const int r = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
                 const uint4 x = *reinterpret_cast<const uint4 *>(stage + at(r, c));
-                if (r < rows) *reinterpret_cast<uint4 *>(base + (size_t)r * M + c * E) = x;
+                if (r < rows && c * E < cols) *reinterpret_cast<uint4 *>(base + (size_t)r * ld + c * E) = x;
             }
-        } else
-            for (int e = lane; e < 32 * W; e += 32) {
-                const int r = e / W, c = e % W;
-                if (r < rows && c < cols) base[(size_t)r * M + c] = *reinterpret_cast<const T *>(stage + at(r, c / E) + c % E * (int)sizeof(T));
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) {
+                const int r = (i * 32 + lane) / ROW_WORDS, k = (i * 32 + lane) % ROW_WORDS, c = k * 4 / (int)sizeof(T);
+                const uint32_t x = *reinterpret_cast<const uint32_t *>(stage + at(r, k / 4) + k % 4 * 4);
+                T *to = base + (size_t)r * ld + c;
+                if (r >= rows || c >= cols) continue;
+                if (sizeof(T) == 4 || align == ALIGN_WORD) *reinterpret_cast<uint32_t *>(to) = x;
+                else {
+                    *reinterpret_cast<unsigned short *>(to) = (unsigned short)x;
+                    if (c + 1 < cols) reinterpret_cast<unsigned short *>(to)[1] = (unsigned short)(x >> 16);
+                }
             }
+        }
         __syncwarp();
     }
     // memory -> registers in two steps, so that the loads can be under way long before the tile is needed
-    static __device__ __forceinline__ void fetch(const T *base, int M, int rows, int cols, bool vec, uint4 (&q)[CHUNKS], int lane)
+    static __device__ __forceinline__ void fetch(const T *base, int ld, int rows, int cols, int align, uint4 (&q)[CHUNKS], int lane)
     {
-        if (!vec || cols < W) return;
 #pragma unroll
-        for (int i = 0; i < CHUNKS; i++) {
-            const int r = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
-            q[i] = make_uint4(0, 0, 0, 0);
-            if (r < rows) q[i] = *reinterpret_cast<const uint4 *>(base + (size_t)r * M + c * E);
+        for (int i = 0; i < CHUNKS; i++) q[i] = make_uint4(0, 0, 0, 0);
+        if (align == ALIGN_16) {
+#pragma unroll
+            for (int i = 0; i < CHUNKS; i++) {
+                const int r = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
+                if (r < rows && c * E < cols) q[i] = *reinterpret_cast<const uint4 *>(base + (size_t)r * ld + c * E);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) {
+                const int r = (i * 32 + lane) / ROW_WORDS, c = (i * 32 + lane) % ROW_WORDS * 4 / (int)sizeof(T);
+                const T *from = base + (size_t)r * ld + c;
+                if (r >= rows || c >= cols) continue;
+                if (sizeof(T) == 4 || align == ALIGN_WORD) word(q, i) = *reinterpret_cast<const uint32_t *>(from);
+                else {
+                    const unsigned short *h = reinterpret_cast<const unsigned short *>(from);
+                    word(q, i) = h[0] | (c + 1 < cols ? (uint32_t)h[1] << 16 : 0u);
+                }
+            }
         }
     }
-    static __device__ __forceinline__ void turn(const T *base, int M, int rows, int cols, bool vec, const uint4 (&q)[CHUNKS], float (&v)[W], unsigned char *stage, int lane)
+    static __device__ __forceinline__ void turn(int align, uint4 (&q)[CHUNKS], float (&v)[W], unsigned char *stage, int lane)
     {
-        if (vec && cols >= W) {
+        if (align == ALIGN_16) {
 #pragma unroll
             for (int i = 0; i < CHUNKS; i++) *reinterpret_cast<uint4 *>(stage + at(i * (32 / CHUNKS) + lane / CHUNKS, lane % CHUNKS)) = q[i];
-        } else
-            for (int e = lane; e < 32 * W; e += 32) {
-                const int r = e / W, c = e % W;
-                if (r < rows && c < cols) *reinterpret_cast<T *>(stage + at(r, c / E) + c % E * (int)sizeof(T)) = base[(size_t)r * M + c];
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) {
+                const int r = (i * 32 + lane) / ROW_WORDS, k = (i * 32 + lane) % ROW_WORDS;
+                *reinterpret_cast<uint32_t *>(stage + at(r, k / 4) + k % 4 * 4) = word(q, i);
             }
+        }
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < CHUNKS; c++) {
@@ -180,26 +212,29 @@ template <class T, int W> struct BmTile {
 };
 // The results of W columns from col on of the 32 rows from row0 on.  v: the accumulators (gate), w: the second ones (up); gq, uq: G and U as BmTile::fetch left them.
 template <class T, int EPI, int W>
-__device__ __forceinline__ void bm_tile_results(const BmJob<T> &p, int row0, int col, float (&v)[W], float (&w)[W], const uint4 (&gq)[BmTile<T, W>::CHUNKS],
-                                                const uint4 (&uq)[BmTile<T, W>::CHUNKS], unsigned char *stage, int lane)
+__device__ __forceinline__ void bm_tile_results(const BmJob<T> &p, int row0, int col, float (&v)[W], float (&w)[W], uint4 (&gq)[BmTile<T, W>::CHUNKS],
+                                                uint4 (&uq)[BmTile<T, W>::CHUNKS], unsigned char *stage, int lane)
 {
     typedef BmTile<T, W> Tile;
     constexpr bool FAST = sizeof(T) == 2;
-    const size_t at = (size_t)row0 * p.M + col;
+    const size_t at = (size_t)row0 * p.ld + col;
     const int rows = p.N - row0, cols = p.M - col;
-    const bool vec = p.vec;
     if constexpr (EPI == FFN_GATE) {
-        if (p.g) { Tile::store(p.g + at, p.M, rows, cols, vec, v, stage, lane); Tile::store(p.u + at, p.M, rows, cols, vec, w, stage, lane); }
+        if (p.g) {
+            const size_t of = (size_t)row0 * p.M + col;
+            Tile::store(p.g + of, p.M, rows, cols, p.g_align, v, stage, lane);
+            Tile::store(p.u + of, p.M, rows, cols, p.g_align, w, stage, lane);
+        }
 #pragma unroll
         for (int j = 0; j < W; j++) v[j] = gate_fw<FAST>(v[j], w[j]);
     } else if constexpr (EPI == FFN_GATE_BW) {
         float g[W], u[W];
-        Tile::turn(p.g + at, p.M, rows, cols, vec, gq, g, stage, lane);
-        Tile::turn(p.u + at, p.M, rows, cols, vec, uq, u, stage, lane);
+        Tile::turn(p.g_align, gq, g, stage, lane);
+        Tile::turn(p.g_align, uq, u, stage, lane);
 #pragma unroll
         for (int j = 0; j < W; j++) { const float dh = v[j]; gate_bw<FAST>(g[j], u[j], dh, v[j], g[j], u[j]); }
-        Tile::store(p.dg + at, p.M, rows, cols, vec, g, stage, lane);
-        Tile::store(p.du + at, p.M, rows, cols, vec, u, stage, lane);
+        Tile::store(p.dg + at, p.ld, rows, cols, p.c_align, g, stage, lane);
+        Tile::store(p.du + at, p.ld, rows, cols, p.c_align, u, stage, lane);
     } else if constexpr (EPI == FFN_INT8) {
         const float xs = ld0(lane < rows, p.xs + row0 + lane);
         const bool even = cols >= W && ((uintptr_t)p.ws & 15) == 0;
@@ -213,30 +248,31 @@ __device__ __forceinline__ void bm_tile_results(const BmJob<T> &p, int row0, int
             for (int j = 0; j < W; j++) v[j] += s[j];
         }
     }
-    Tile::store(p.C + at, p.M, rows, cols, vec, v, stage, lane);
+    Tile::store(p.C + at, p.ld, rows, cols, p.c_align, v, stage, lane);
 }
 // The same for four columns of a row (from partial tiles)
 template <class T, int EPI> __device__ __forceinline__ void bm_results(const BmJob<T> &p, int row, int col, float (&v)[4], float (&w)[4])
 {
     constexpr bool FAST = sizeof(T) == 2;
-    const size_t at = (size_t)row * p.M + col;
+    const size_t at = (size_t)row * p.ld + col, of = (size_t)row * p.M + col;
     const int live = p.M - col;
+    const bool c_vec = p.c_align == ALIGN_16, g_vec = p.g_align == ALIGN_16;
     if constexpr (EPI == FFN_GATE) {
-        if (p.g) { bm_st<4>(p.g + at, v, live, p.vec); bm_st<4>(p.u + at, w, live, p.vec); }
+        if (p.g) { bm_st<4>(p.g + of, v, live, g_vec); bm_st<4>(p.u + of, w, live, g_vec); }
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = gate_fw<FAST>(v[j], w[j]);
     } else if constexpr (EPI == FFN_GATE_BW) {
         float g[4], u[4];
-        bm_ld<4>(p.g + at, g, live, p.vec); bm_ld<4>(p.u + at, u, live, p.vec);
+        bm_ld<4>(p.g + of, g, live, g_vec); bm_ld<4>(p.u + of, u, live, g_vec);
 #pragma unroll
         for (int j = 0; j < 4; j++) { const float dh = v[j]; gate_bw<FAST>(g[j], u[j], dh, v[j], g[j], u[j]); }
-        bm_st<4>(p.dg + at, g, live, p.vec); bm_st<4>(p.du + at, u, live, p.vec);
+        bm_st<4>(p.dg + at, g, live, c_vec); bm_st<4>(p.du + at, u, live, c_vec);
     } else if constexpr (EPI == FFN_INT8) {
         const float xs = p.xs[row];
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = v[j] * xs * ld0(j < live, p.ws + col + j) + ld0(p.bias && j < live, p.bias + col + j);
     }
-    bm_st<4>(p.C + at, v, live, p.vec);
+    bm_st<4>(p.C + at, v, live, c_vec);
 }
 
 // tile -> row block, column block: eight row blocks share a sweep over the columns
@@ -461,8 +497,8 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                 if constexpr (EPI == FFN_GATE_BW) {
                     if (!whole || row0 >= j.N || c >= CW || col0 + c >= j.M) return;
                     const size_t at = (size_t)row0 * j.M + col0 + c;
-                    Tile::fetch(j.g + at, j.M, j.N - row0, j.M - col0 - c, j.vec, g1, lane);
-                    Tile::fetch(j.u + at, j.M, j.N - row0, j.M - col0 - c, j.vec, u1, lane);
+                    Tile::fetch(j.g + at, j.M, j.N - row0, j.M - col0 - c, j.g_align, g1, lane);
+                    Tile::fetch(j.u + at, j.M, j.N - row0, j.M - col0 - c, j.g_align, u1, lane);
                 }
             };
             uint32_t *mine = j.part + ((size_t)(un.tile * j.splits + un.rank) * BM_ROWS + row_in) * BN;        // row of the partial tile (splits > 1)
@@ -556,12 +592,16 @@ template <int KIND, int BN> __device__ __forceinline__ void bm_add_parts(const u
         for (int k = 0; k < splits; k++) { const float4 x = *reinterpret_cast<const float4 *>(from + (size_t)k * BM_ROWS * BN); t[0] += x.x; t[1] += x.y; t[2] += x.z; t[3] += x.w; }
     }
 }
-// The results from the partial tiles of a split contraction: a thread per four neighbouring results, partial tiles added in order.
-template <int KIND, class T, int EPI, int BN> __global__ void __launch_bounds__(256) bm_reduce_kernel(const __grid_constant__ BmJob<T> p)
+// The results from the partial tiles of the launch's split contractions: a thread per four neighbouring results, partial tiles added in order.
+template <int KIND, class T, int EPI, int BN> __global__ void __launch_bounds__(256) bm_reduce_kernel(const __grid_constant__ BmParams<T, bm_jobs(EPI)> all)
 {
     pdl_wait();
+    int job = 0;
+#pragma unroll
+    for (int k = 1; k < bm_jobs(EPI); k++) if (k < all.jobs && (int)blockIdx.x >= all.job[k].reduce_first) job = k;        // (one that is not split has no blocks: the next one starts there too)
+    const BmJob<T> &p = all.job[job];
     constexpr int BNC = EPI == FFN_GATE ? BN / 2 : BN, QUADS = BNC / 4, PER = BM_ROWS * QUADS;       // (PER is a multiple of 256: a block stays inside one tile)
-    const int e = blockIdx.x * 256 + threadIdx.x, tile = e / PER, in = e - tile * PER, r = in / QUADS, c = (in - r * QUADS) * 4;
+    const int block = (int)blockIdx.x - p.reduce_first, tile = block / (PER / 256), e = (block % (PER / 256) + tile * (PER / 256)) * 256 + threadIdx.x, in = e - tile * PER, r = in / QUADS, c = (in - r * QUADS) * 4;
     int rb, cb;
     bm_locate(p, tile, rb, cb);
     const int row = rb * BM_ROWS + r, col = cb * BNC + c;
@@ -597,7 +637,7 @@ template <class T, int JOBS> static BmPlan bm_plan(int kind, int epi, BmParams<T
     for (int i = kind == MM_TF32 ? 1 : 0; i < (kind == MM_TF32 ? 3 : 4); i++) {
         const bool two = i == 3;
         const int bn = bns[i], bnc = epi == FFN_GATE ? bn / 2 : bn, places = two ? sm_count() / 2 : sm_count();
-        int splits[JOBS], tiles[JOBS], units = 0;
+        int splits[JOBS] = {}, tiles[JOBS] = {}, units = 0;
         for (int k = 0; k < p.jobs; k++) { splits[k] = 1; units += tiles[k] = ceil_div(p.job[k].N, two ? 256 : 128) * ceil_div(p.job[k].M, bnc); }
         const double tensor = (kind == MM_TF32 ? 6.0 : 2.0) * bn * (two ? 4.0 / 3.0 : 1.0);
         for (;;) {
@@ -634,9 +674,7 @@ template <int KIND, class T, int EPI, int BN, bool PAIR> static void bm_launch(c
     if constexpr (PAIR) TL_LAUNCH_CLUSTER((block_mm_kernel<KIND, T, EPI, BN, PAIR>), (unsigned)(2 * std::min(p.units, sm_count() / 2)), BM_THREADS, smem, 2, maps, p);
     else {
         TL_LAUNCH((block_mm_kernel<KIND, T, EPI, BN, PAIR>), (unsigned)std::min(p.units, sm_count()), BM_THREADS, smem, maps, p);
-        for (int k = 0; k < p.jobs; k++)
-            if (p.job[k].splits > 1)
-                TL_LAUNCH((bm_reduce_kernel<KIND, T, EPI, BN>), (unsigned)((long long)p.job[k].tiles_m * p.job[k].tiles_n * BM_ROWS * (EPI == FFN_GATE ? BN / 2 : BN) / 4 / 256), 256, 0, p.job[k]);
+        if (p.reduce_blocks) TL_LAUNCH((bm_reduce_kernel<KIND, T, EPI, BN>), (unsigned)p.reduce_blocks, 256, 0, p);
     }
 }
 template <int KIND, class T, int EPI> static void bm_dispatch(const BmPlan &plan, const BmMapList<bm_jobs(EPI)> &maps, const BmParams<T, bm_jobs(EPI)> &p)
@@ -655,17 +693,24 @@ template <int KIND, class T, int EPI> static bool bm_setup(Scope &sc, const BmPl
     p.status = tc_status_word();
     p.stage_bytes = BmCfg<KIND>::PARTS * (BM_ROWS * 128u + (uint32_t)(plan.pair ? plan.BN / 2 : plan.BN) * 128u);
     p.stages = std::min<int>(BM_MAX_STAGES, BM_RING / p.stage_bytes);
-    p.units = 0;
+    p.units = p.reduce_blocks = 0;
     for (int k = 0; k < p.jobs; k++) {
         BmJob<T> &j = p.job[k];
+        j.reduce_first = p.reduce_blocks;
         j.tiles_m = ceil_div(j.M, bnc); j.tiles_n = ceil_div(j.N, plan.pair ? 2 * BM_ROWS : BM_ROWS);
         j.first = p.units;
         p.units += j.tiles_m * j.tiles_n * j.splits;
+        if (j.splits > 1) p.reduce_blocks += j.tiles_m * j.tiles_n * (BM_ROWS * bnc / 4 / 256);
         if (j.splits > 1 && !(j.part = sc.scratch<uint32_t>((size_t)j.tiles_m * j.tiles_n * j.splits * BM_ROWS * plan.BN))) return false;
     }
     return p.status != nullptr;
 }
 
+template <class T> static int bm_align(int ld, const void *a, const void *b, const void *c)
+{
+    const uintptr_t at = (uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)((size_t)ld * sizeof(T));
+    return at % 16 == 0 ? ALIGN_16 : at % 4 == 0 ? ALIGN_WORD : ALIGN_ELEMENT;
+}
 static bool bm_ready()
 {
     if (tc_encode_tiled_fn()) return true;
@@ -692,16 +737,18 @@ template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> *list, 
     constexpr long long EB = 16 / (long long)sizeof(T);
     if (!bm_ready()) return false;
     // what takes longest goes first
-    const FfnProduct<T> *order[JOBS];
+    const FfnProduct<T> *order[JOBS] = {};
     for (int k = 0; k < count; k++) order[k] = list + k;
-    std::sort(order, order + count, [](const FfnProduct<T> *x, const FfnProduct<T> *y) { return (long long)x->K * x->terms > (long long)y->K * y->terms; });
+    auto length = [](const FfnProduct<T> *f) { return (long long)f->K * f->terms; };
+    for (int k = 1; k < count; k++)
+        for (int i = k; i > 0 && length(order[i]) > length(order[i - 1]); i--) std::swap(order[i], order[i - 1]);
     struct Op { const T *at; long long os, ps; int mn; };
     struct Done { const T *src; long long rs, cs; int rows, K; Op op; } done[12];
     BmPacks<T> pack;
     pack.count = pack.blocks = 0;
     // one layout for all operands of a side: they share strides, and all are read in place or none.  An operand of two products is copied once.
     auto side = [&](const T *const *src, int n, long long rs, long long cs, int rows, int K, Op *o) -> bool {
-        const int Kp = (int)(((long long)K + EB - 1) / EB * EB);
+        const int Kp = (int)(((long long)K + 8 * EB - 1) / (8 * EB) * (8 * EB));           // (whole lines: a box's 128 bytes over two of them are fetched as two)
         int where = tm_in_place<T>(src[0], rs, cs, 0, rows, K, 1);
         if (n > 1 && tm_in_place<T>(src[1], rs, cs, 0, rows, K, 1) != where) where = 0;
         for (int i = 0; i < n; i++) {
@@ -725,15 +772,14 @@ template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> *list, 
     Op a[JOBS][2], b[JOBS][2];
     BmParams<T, JOBS> p = {};
     p.jobs = count;
-    auto odd = [](const void *q) { return ((uintptr_t)q & 15) != 0; };
     for (int k = 0; k < count; k++) {
         const FfnProduct<T> &f = *order[k];
         BmJob<T> &j = p.job[k];
         if (!side(f.A, f.terms, f.a_rs, f.a_cs, f.N, f.K, a[k]) || !side(f.B, EPI == FFN_GATE ? 2 : f.terms, f.b_cs, f.b_rs, f.M, f.K, b[k])) return false;
-        j.C = f.C; j.g = f.g; j.u = f.u; j.dg = f.dg; j.du = f.du; j.N = f.N; j.M = f.M;
+        j.C = f.C; j.g = f.g; j.u = f.u; j.dg = f.dg; j.du = f.du; j.N = f.N; j.M = f.M; j.ld = f.ld;
         j.kps = ceil_div(f.K, BK); j.ksteps = j.kps * f.terms;
         j.a_mn = a[k][0].mn; j.b_mn = b[k][0].mn;
-        j.vec = f.M % EB == 0 && !odd(f.C) && !odd(f.g) && !odd(f.u) && !odd(f.dg) && !odd(f.du);
+        j.c_align = bm_align<T>(f.ld, f.C, f.dg, f.du); j.g_align = bm_align<T>(f.M, f.g, f.u, nullptr);
     }
     const BmPlan plan = bm_plan<T, JOBS>(KIND, EPI, p);
     if (!bm_setup<KIND, T, EPI>(sc, plan, p)) return false;
@@ -759,8 +805,9 @@ template <class T, int EPI> bool block_mm(Scope &sc, const FfnProduct<T> *list, 
 INST(float)
 INST(__half)
 
-// Rows of `size` bytes that do not lie on 16-byte boundaries -> rows of `quads` 16-byte groups (behind the end: never read), of both operands; a thread per group
-struct BmRows { const signed char *src[2]; uint4 *dst[2]; long long groups[2]; };
+// Rows of `size` bytes that do not lie on 16-byte boundaries -> rows of `quads` 16-byte groups (behind the end: never read), of both operands; a thread per group,
+// from the five words around its bytes (2338 rows of 7772 bytes and 192: 14.8 us byte by byte).
+struct BmRows { const unsigned char *src[2], *end[2]; uint4 *dst[2]; long long groups[2]; };
 __global__ void __launch_bounds__(256) pack_rows_int8_kernel(const __grid_constant__ BmRows p, int size, int quads)
 {
     pdl_wait();
@@ -770,17 +817,29 @@ __global__ void __launch_bounds__(256) pack_rows_int8_kernel(const __grid_consta
     if (e >= p.groups[which]) return;
     const long long r = e / quads;
     const int k = (int)(e - r * quads) * 16;
-    const signed char *s = p.src[which] + (size_t)r * size + k;
-    uint32_t w[4] = {0, 0, 0, 0};
+    if (k >= size) return;
+    const unsigned char *s = p.src[which] + (size_t)r * size + k, *begin = p.src[which], *end = p.end[which];
+    const int off = (int)((uintptr_t)s & 3);
+    uint32_t v[5], w[4];
 #pragma unroll
-    for (int b = 0; b < 16; b++) if (k + b < size) w[b / 4] |= (uint32_t)(unsigned char)s[b] << (8 * (b % 4));
+    for (int i = 0; i < 5; i++) {
+        const unsigned char *a = s - off + 4 * i;
+        v[i] = 0;
+        if (a >= begin && a + 4 <= end) v[i] = *reinterpret_cast<const uint32_t *>(a);
+        else {
+#pragma unroll
+            for (int b = 0; b < 4; b++) if (a + b >= begin && a + b < end) v[i] |= (uint32_t)a[b] << (8 * b);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * off);
     p.dst[which][e] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <class T> void linear_int8(Scope &sc, const signed char *x, const float *xs, const signed char *w, const float *ws, const T *bias, T *y, int rows, int in, int out)
 {
     if (rows <= FEW_ROWS) return few_rows_int8<T>(sc, x, xs, w, ws, bias, y, rows, in, out);
     if (!bm_ready()) return;
-    const int quads = ceil_div(in, 16);
+    const int quads = ceil_div(in, 128) * 8;                 // (whole lines, as above)
     const signed char *at[2] = {x, w};
     signed char *copy[2] = {nullptr, nullptr};
     const int count[2] = {rows, out};
@@ -791,9 +850,9 @@ template <class T> void linear_int8(Scope &sc, const signed char *x, const float
     BmParams<T, 1> p = {};
     BmJob<T> &j = p.job[0];
     p.jobs = 1;
-    j.C = y; j.bias = bias; j.xs = xs; j.ws = ws; j.N = rows; j.M = out;
+    j.C = y; j.bias = bias; j.xs = xs; j.ws = ws; j.N = rows; j.M = j.ld = out;
     j.kps = j.ksteps = ceil_div(in, BmCfg<MM_I8>::BK);
-    j.vec = out % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)y & 15) == 0;
+    j.c_align = bm_align<T>(out, y, nullptr, nullptr);
     const BmPlan plan = bm_plan<T, 1>(MM_I8, FFN_INT8, p);
     if (!bm_setup<MM_I8, T, FFN_INT8>(sc, plan, p)) return;
     BmMapList<1> maps;
@@ -802,7 +861,7 @@ template <class T> void linear_int8(Scope &sc, const signed char *x, const float
                     i ? (plan.pair ? plan.BN / 2 : plan.BN) : BM_ROWS)) { bm_no_map(); return; }
     if (copy[0] || copy[1]) {
         BmRows q;
-        for (int i = 0; i < 2; i++) { q.src[i] = at[i]; q.dst[i] = (uint4 *)copy[i]; q.groups[i] = copy[i] ? (long long)count[i] * quads : 0; }
+        for (int i = 0; i < 2; i++) { q.src[i] = (const unsigned char *)at[i]; q.end[i] = q.src[i] + (size_t)count[i] * in; q.dst[i] = (uint4 *)copy[i]; q.groups[i] = copy[i] ? (long long)count[i] * quads : 0; }
         TL_LAUNCH(pack_rows_int8_kernel, ceil_div(q.groups[0] + q.groups[1], 256), 256, 0, q, in, quads);
     }
     bm_dispatch<MM_I8, T, FFN_INT8>(plan, maps, p);

@@ -20,14 +20,15 @@ template <bool FAST> __device__ __forceinline__ void gate_bw(float g, float u, f
     dg = dh * u * fmaf(a, 1.f - s, s);
 }
 
-// C(i, j) = sum_k A(i, k) B(k, j), i < N, j < M, k < K; A(i, k) = A[i * a_rs + k * a_cs], B(k, j) = B[k * b_rs + j * b_cs], results dense.
+// C(i, j) = sum_k A(i, k) B(k, j), i < N, j < M, k < K; A(i, k) = A[i * a_rs + k * a_cs], B(k, j) = B[k * b_rs + j * b_cs],
+// C, dg and du in rows of ld elements (padding is written where ld covers it), g and u dense.
 //   FFN_PLAIN: C = the sum over `terms` (1 or 2) pairs of operands;  FFN_GATE: g, u (may be null) = A[0] with B[0] and B[1], C = silu(g) * u;
 //   FFN_GATE_BW: dH = A[0] B[0]; reads g and u, writes C = silu(g) * u and their gradients dg, du
 enum { FFN_PLAIN = 0, FFN_GATE = 1, FFN_GATE_BW = 2, FFN_INT8 = 3 };
 template <class T> struct FfnProduct {
     const T *A[2], *B[2];
     T *C, *g, *u, *dg, *du;
-    int N, M, K, terms;
+    int N, M, K, terms, ld;
     long long a_rs, a_cs, b_rs, b_cs;
 };
 // On the tensor cores (tl_block_mm.cu); false: nothing launched, the error is set (no memory for an operand's copy, no tensor-map encoder)
