@@ -45,15 +45,33 @@ template <class T, int JOBS> struct BmParams {
 struct BmMaps { CUtensorMap a[2], b[2]; };
 template <int JOBS> struct BmMapList { BmMaps of[JOBS]; };
 
-// D = A B^T of 8-bit integers, 32 bytes of K
-template <bool PAIR> __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+// The four MMAs of a stage, 32 bytes (or 16 rows) of K each; a, b: lower words of the first one's descriptors, SA, SB: 16-byte units to the next one's.  What the
+// issuing thread does per stage decides where tiles are small: with 64-bit descriptors added up, steps in registers and the barrier asked only when its stage
+// was wanted a stage took 490 cycles (128 x 64 of 8 bits: 128 on the tensor cores).
+constexpr uint32_t BM_DESC_UPPER = 1024u >> 4 | 1u << 14 | LAYOUT_SW128 << 29;
+#define TL_BM_MMA(GROUP, TYPE, ACC) \
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t" ACC "add.u32 la, %1, %4;\n\tadd.u32 lb, %2, %5;\n\t" \
+                 "mov.b64 da, {la, %6};\n\tmov.b64 db, {lb, %6};\n\ttcgen05.mma.cta_group::" GROUP ".kind::" TYPE " [%0], da, db, %3, p;\n\t}" \
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "n"(kk * SA), "n"(kk * SB), "n"(BM_DESC_UPPER), "r"(acc) : "memory")
+#define TL_BM_MMA_KIND(ACC)                                                                                   \
+    do {                                                                                                      \
+        if constexpr (KIND == MM_F16) { if constexpr (PAIR) TL_BM_MMA("2", "f16", ACC); else TL_BM_MMA("1", "f16", ACC); }         \
+        else if constexpr (KIND == MM_TF32) { if constexpr (PAIR) TL_BM_MMA("2", "tf32", ACC); else TL_BM_MMA("1", "tf32", ACC); } \
+        else { if constexpr (PAIR) TL_BM_MMA("2", "i8", ACC); else TL_BM_MMA("1", "i8", ACC); }               \
+    } while (0)
+template <int KIND, bool PAIR, int SA, int SB, int kk> __device__ __forceinline__ void bm_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc)
 {
-    if constexpr (PAIR)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+    if constexpr (kk == 0) TL_BM_MMA_KIND("setp.ne.b32 p, %7, 0;\n\t");
+    else TL_BM_MMA_KIND("setp.eq.b32 p, 0, 0;\n\t");
+}
+#undef TL_BM_MMA_KIND
+#undef TL_BM_MMA
+template <int KIND, bool PAIR, int SA, int SB> __device__ __forceinline__ void bm_step(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc)
+{
+    bm_mma<KIND, PAIR, SA, SB, 0>(d, a, b, idesc, acc);
+    bm_mma<KIND, PAIR, SA, SB, 1>(d, a, b, idesc, acc);
+    bm_mma<KIND, PAIR, SA, SB, 2>(d, a, b, idesc, acc);
+    bm_mma<KIND, PAIR, SA, SB, 3>(d, a, b, idesc, acc);
 }
 // accumulators of 32-bit integers (2), operands of signed 8 bits (1), both K-major
 __host__ __device__ constexpr uint32_t i8_idesc(uint32_t M, uint32_t N) { return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24); }
@@ -146,18 +164,19 @@ template <class T, int W> struct BmTile {
                 const uint4 x = *reinterpret_cast<const uint4 *>(stage + at(r, c));
                 if (r < rows && c * E < cols) *reinterpret_cast<uint4 *>(base + (size_t)r * ld + c * E) = x;
             }
-        } else {
+        } else if (sizeof(T) == 4 || align == ALIGN_WORD) {
 #pragma unroll
             for (int i = 0; i < WORDS; i++) {
                 const int r = (i * 32 + lane) / ROW_WORDS, k = (i * 32 + lane) % ROW_WORDS, c = k * 4 / (int)sizeof(T);
                 const uint32_t x = *reinterpret_cast<const uint32_t *>(stage + at(r, k / 4) + k % 4 * 4);
-                T *to = base + (size_t)r * ld + c;
-                if (r >= rows || c >= cols) continue;
-                if (sizeof(T) == 4 || align == ALIGN_WORD) *reinterpret_cast<uint32_t *>(to) = x;
-                else {
-                    *reinterpret_cast<unsigned short *>(to) = (unsigned short)x;
-                    if (c + 1 < cols) reinterpret_cast<unsigned short *>(to)[1] = (unsigned short)(x >> 16);
-                }
+                if (r < rows && c < cols) *reinterpret_cast<uint32_t *>(base + (size_t)r * ld + c) = x;
+            }
+        } else {                                             // (neighbouring elements from neighbouring lanes: halves of words alternating would be two writes of every sector)
+#pragma unroll 8
+            for (int i = 0; i < W; i++) {
+                const int r = (i * 32 + lane) / W, c = (i * 32 + lane) % W;
+                const T x = *reinterpret_cast<const T *>(stage + at(r, c / E) + c % E * (int)sizeof(T));
+                if (r < rows && c < cols) base[(size_t)r * ld + c] = x;
             }
         }
         __syncwarp();
@@ -398,7 +417,9 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                 for (int i = 0; i < 100000 && !mbar_try_wait(&full[j], parity); i++) __nanosleep(100);
             }
     } else if (warp == BM_EPI + 1) {
-        if (!PAIR || rank == 0) {
+        if ((!PAIR || rank == 0) && elect_one()) {                                // one thread walks the loop
+            const uint32_t stage_step = p.stage_bytes >> 4;
+            bool ready = false;                                                     // the next stage was seen full
             const uint32_t idesc_lo = mma_idesc(FMT_TF32, ROWS, BN);
             int s = 0, it = 0;
             uint32_t phase = 0;
@@ -408,10 +429,9 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                 const bool a_mn = KIND == MM_F16 && p.job[un.job].a_mn, b_mn = KIND == MM_F16 && p.job[un.job].b_mn;
                 const uint32_t majors = (a_mn ? IDESC_A_MN_MAJOR : 0u) | (b_mn ? IDESC_B_MN_MAJOR : 0u);
                 const uint32_t idesc = KIND == MM_F16 ? (mma_idesc(FMT_F16, ROWS, BN) | majors) : KIND == MM_I8 ? i8_idesc(ROWS, BN) : mma_idesc(FMT_TF32, ROWS, 2 * BN);
-                // descriptor words that do not depend on the stage, and the step of one MMA (32 bytes or 16 rows of K) in 16-byte units
-                const uint64_t desc_a = a_mn ? smem_desc_swizzled(0, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(0, 1024);
-                const uint64_t desc_b = b_mn ? smem_desc_swizzled(0, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(0, 1024);
-                const uint32_t step_a = a_mn ? 128u : 2u, step_b = b_mn ? 128u : 2u;
+                // lower descriptor words of stage 0 (the upper one is the same in every layout used)
+                const uint32_t low_a = (uint32_t)(a_mn ? smem_desc_swizzled(sbase, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(sbase, 1024));
+                const uint32_t low_b = (uint32_t)(b_mn ? smem_desc_swizzled(sbase + PARTS * A_BYTES, 8192u, 1024u, LAYOUT_SW128) : smem_desc_kmajor_sw128(sbase + PARTS * A_BYTES, 1024));
                 for (int kc = un.ks0; kc < un.ks1 && ok; it++) {
                     const int kend = KIND == MM_TF32 ? min(un.ks1, kc + BM_CHUNK) : un.ks1, buf = it % NBUF, use = it / NBUF;
                     if (use > 0 && !tm_wait(&acc_empty[buf], (uint32_t)(use - 1) & 1u, failed)) { ok = false; break; }
@@ -419,33 +439,29 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                     const uint32_t d = tmem + buf * BUF_COLS;
                     uint32_t acc = 0;
                     for (; kc < kend; kc++) {
-                        if (!tm_wait(&full[s], phase, failed)) { ok = false; break; }
-                        tc_fence_after();
-                        if (elect_one()) {
-                            const uint32_t st = sbase + s * p.stage_bytes, sb = st + PARTS * A_BYTES;
-                            const uint64_t da = desc_a + (st >> 4), db = desc_b + (sb >> 4);
-#pragma unroll
-                            for (int kk = 0; kk < 4; kk++) {                        // 4 MMAs of 32 bytes of K each per 128-byte row
-                                if constexpr (KIND == MM_I8) mma_i8<PAIR>(d, da + kk * step_a, db + kk * step_b, idesc, kk ? 1u : acc);
-                                else tm_mma<KIND == MM_F16, PAIR>(d, da + kk * step_a, db + kk * step_b, idesc, kk ? 1u : acc);
-                                if constexpr (KIND == MM_TF32) tm_mma<false, PAIR>(d + 2 * BN, da + (A_BYTES >> 4) + kk * step_a, db + kk * step_b, idesc_lo, kk ? 1u : acc);
-                            }
-                            tm_commit<PAIR>(&empty[s]);
-                        }
-                        __syncwarp();
-                        acc = 1u;
+                        if (!ready && !tm_wait(&full[s], phase, failed)) { ok = false; break; }
+                        const int now = s;
                         if (++s == ST) { s = 0; phase ^= 1u; }
+                        ready = mbar_try_wait(&full[s], phase);                 // of the next step: its answer comes while this one's MMAs are issued
+                        tc_fence_after();
+                        const uint32_t a = low_a + now * stage_step, b = low_b + now * stage_step;
+                        if (KIND != MM_F16 || !(a_mn || b_mn)) bm_step<KIND, PAIR, 2, 2>(d, a, b, idesc, acc);
+                        else if (a_mn && b_mn) bm_step<KIND, PAIR, 128, 128>(d, a, b, idesc, acc);
+                        else if (b_mn) bm_step<KIND, PAIR, 2, 128>(d, a, b, idesc, acc);
+                        else bm_step<KIND, PAIR, 128, 2>(d, a, b, idesc, acc);
+                        if constexpr (KIND == MM_TF32) bm_step<KIND, PAIR, 2, 2>(d + 2 * BN, a + (A_BYTES >> 4), b, idesc_lo, acc);
+                        tm_commit<PAIR>(&empty[now]);
+                        acc = 1u;
                     }
-                    if (ok && elect_one()) tm_commit<PAIR>(&acc_full[buf]);
-                    __syncwarp();
+                    if (ok) tm_commit<PAIR>(&acc_full[buf]);
                 }
             }
             if (!ok) {                                                              // given up: what was issued ends first
-                if (elect_one()) tm_commit<PAIR>(&last_bar);
-                __syncwarp();
+                tm_commit<PAIR>(&last_bar);
                 for (int i = 0; i < 100000 && !mbar_try_wait(&last_bar, 0); i++) __nanosleep(100);
             }
         }
+        __syncwarp();
     } else {
         // epilogue: warp w owns TMEM lanes 32 (w % 4) .. + 31, one row each, and one half of the tile's result columns
         const int quarter = warp & 3, half = warp >> 2;
@@ -624,9 +640,9 @@ static bool bm_map(CUtensorMap *m, CUtensorMapDataType type, int esize, const vo
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tile and CTAs per tile with the fewest cycles by the model that the plain products use (tl_gemm_tma.cu): a K step costs its tensor time or
-// what its bytes take from L2 into an SM (58 bytes per cycle with every SM loading, 81 with half of them), a pair's a third more than its tensor
-// time; a tile 2500 cycles beside its K steps, a launch 2000 (pairs 10000), partial tiles a launch and their bytes.
+// Tile and CTAs per tile with the fewest cycles by a model: a K step costs its tensor time or what its bytes take into an SM (58 per cycle with several tiles for
+// every SM, 100 with one at most: its shared memory feeds the tensor cores no faster), a pair's a third more than its tensor time; a tile 1000 cycles beside its K
+// steps, a launch 2000 (pairs 8000), partial tiles 2000 and their bytes.  On 38 products of 64 to 4096 rows, timed with every tile and up to 16 parts, what it takes is 0.8% slower than the fastest on average.
 struct BmPlan { int BN, pair; };
 // Several products in one launch: the sum of their units' cycles over the CTAs and the longest unit, for which a product's K is split while CTAs are idle.
 template <class T, int JOBS> static BmPlan bm_plan(int kind, int epi, BmParams<T, JOBS> &p)
@@ -641,17 +657,17 @@ template <class T, int JOBS> static BmPlan bm_plan(int kind, int epi, BmParams<T
         for (int k = 0; k < p.jobs; k++) { splits[k] = 1; units += tiles[k] = ceil_div(p.job[k].N, two ? 256 : 128) * ceil_div(p.job[k].M, bnc); }
         const double tensor = (kind == MM_TF32 ? 6.0 : 2.0) * bn * (two ? 4.0 / 3.0 : 1.0);
         for (;;) {
-            const double fill = (kind == MM_TF32 ? 2 : 1) * 128.0 * (128 + (two ? bn / 2 : bn)) / (units <= places / 2 ? 81.0 : 58.0), step = std::max(tensor, fill);
+            const double fill = (kind == MM_TF32 ? 2 : 1) * 128.0 * (128 + (two ? bn / 2 : bn)) / (units <= places ? 100.0 : 58.0), step = std::max(tensor, fill);
             double sum = 0, longest = 0, reduce = 0;
             int at = 0;
             for (int k = 0; k < p.jobs; k++) {
-                const double unit = step * ceil_div(p.job[k].ksteps, splits[k]) + 2500.0;
+                const double unit = step * ceil_div(p.job[k].ksteps, splits[k]) + 1000.0;
                 sum += unit * tiles[k] * splits[k];
                 if (unit > longest) { longest = unit; at = k; }
-                if (splits[k] > 1) reduce += 4000.0 + 512.0 * bn * tiles[k] * splits[k] / 2000.0;
+                if (splits[k] > 1) reduce += 2000.0 + 512.0 * bn * tiles[k] * splits[k] / 2000.0;
             }
             const double work = p.jobs == 1 ? ceil_div(units, places) * longest : std::max(sum / places + 0.3 * longest, longest);
-            const double cost = (two ? 10000.0 : 2000.0) + work + reduce;
+            const double cost = (two ? 8000.0 : 2000.0) + work + reduce;
             if (cost < 0.97 * best) { best = cost; plan = {bn, two ? 1 : 0}; for (int k = 0; k < p.jobs; k++) p.job[k].splits = splits[k]; }
             // alone, a product's parts have to fit the CTAs once; among others, parts shorten the unit that the launch would wait for
             const bool more = p.jobs == 1 ? units + tiles[at] <= places : longest > 0.5 * sum / places && (long long)tiles[at] * (splits[at] + 1) * BM_ROWS * bn <= (16ll << 20);
