@@ -319,7 +319,6 @@ template <class T, int JOBS> __device__ __forceinline__ BmUnit bm_unit(const BmP
 template <int KIND, class T, int EPI, int BN, bool PAIR>
 __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_constant__ BmMapList<bm_jobs(EPI)> maps, const __grid_constant__ BmParams<T, bm_jobs(EPI)> p)
 {
-    pdl_wait();
     constexpr int BK = BmCfg<KIND>::BK, PARTS = BmCfg<KIND>::PARTS;
     constexpr int BNL = PAIR ? BN / 2 : BN;                                         // rows of B in this CTA's shared memory
     constexpr int BNC = EPI == FFN_GATE ? BN / 2 : BN;                              // result columns of a tile
@@ -361,6 +360,7 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    pdl_wait();
     if (warp == BM_EPI) {
         // producer (whole warp; a thread is elected around the instructions)
         const uint32_t full0 = PAIR ? tm_mapa(smem_u32(&full[0]), 0) : 0u;          // the pair's leader counts both CTAs' bytes
