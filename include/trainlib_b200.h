@@ -119,7 +119,9 @@ void  trainlib_gelu_fp16_bw_cl(void *act_args_fp16);
  *          dx = dsum + r * (g - h * r^2 * mean(g * h)) is the gradient of x and of residual; dsum (NULL: none) is the gradient that
  *          reaches the sum along the residual path.  dweight[j] = sum over the rows of dy * h * r.  dx or dweight may be NULL (not
  *          wanted), not both.  dx may be dy, dsum or sum itself.
- * Every row is reduced in one fixed order and so are the rows of dweight: results are the same bits every time. */
+ * The sum of a row's squares is a float: where it overflows, r is 0 (results of 0, in 8 bits a scale that is NaN).
+ * Every row is reduced in one fixed order and so are the rows of dweight: a call repeated gives the same bits (the order depends on
+ * the sizes and on whether all tensors start on 16 bytes). */
 struct trainlib_rmsnorm_args {
     void *x; void *residual; void *weight; void *sum; void *output;
     signed char *q; float *scale;
@@ -138,8 +140,12 @@ void  trainlib_rmsnorm_fp16_bw_cl(void *trainlib_rmsnorm_args);
  *   fw:  reads x and the weights, writes y; gate and up, both or neither, receive the projections for a backward pass.
  *   bw:  reads dy, gate and up (as the forward pass left them) and what the wanted gradients need: w_down for dx, dw_gate and
  *        dw_up; w_gate and w_up for dx; x for dw_gate and dw_up.  Any of dx, dw_gate, dw_up, dw_down may be NULL (not wanted), not all.
- * The product silu(gate) * up and its gradients are library scratch of `rows * hidden` elements each: three of them in the backward
- * pass.  In fp16 they are rounded to fp16 between the products (what passes 65504 there is infinite).  Outputs must not overlap inputs. */
+ * The product silu(gate) * up and its gradients are library scratch of `rows * hidden` elements each (`hidden` rounded up to 128
+ * bytes): three of them in the backward pass; beside them copies of operands whose rows do not start on 16 bytes, in fp32 of every
+ * operand twice, and partial sums of up to 64 MB.  In fp16 silu(gate) * up and the gradients are rounded to fp16 between the products
+ * (what passes 65504 there is infinite); up to eight rows of a forward pass it goes on unrounded.  A call repeated gives the same bits;
+ * rows, alignment and which gradients are asked for together may change the order of a sum.  Outputs must not overlap inputs.  A size
+ * above 2^30 is refused (TL_ERR_TOO_LARGE). */
 struct trainlib_gated_ffn_args {
     void *x; void *w_gate; void *w_up; void *w_down; void *gate; void *up; void *y;
     int rows; int in_size; int hidden; int out_size;

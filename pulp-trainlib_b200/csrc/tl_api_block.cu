@@ -1,6 +1,7 @@
 // Entry points of the feed-forward half of a transformer block: RMS norm of a residual sum, gated feed-forward block, linear layer in
 // 8-bit integers.  Same conventions as the other entry points: host pointers are staged, device pointers pass through, errors latch.
 #include "tl_kernels.h"
+#include <algorithm>
 
 using namespace tl;
 
@@ -66,7 +67,12 @@ template <class T> void linear_int8_impl(void *args)
 }
 template <class T> bool gated_ffn_sizes(trainlib_gated_ffn_args *a)
 {
-    if (a && a->rows > 0 && a->in_size > 0 && a->hidden > 0 && a->out_size > 0) return true;
+    if (a && a->rows > 0 && a->in_size > 0 && a->hidden > 0 && a->out_size > 0) {
+        const int largest = std::max(std::max(a->rows, a->in_size), std::max(a->hidden, a->out_size));
+        if (largest <= 1 << 30) return true;
+        set_error(TL_ERR_TOO_LARGE, "trainlib_gated_ffn: a size of %d, 2^30 at most", largest);
+        return false;
+    }
     set_error(TL_ERR_BAD_ARGS, "trainlib_gated_ffn: rows=%d in_size=%d hidden=%d out_size=%d", a ? a->rows : 0, a ? a->in_size : 0, a ? a->hidden : 0, a ? a->out_size : 0);
     return false;
 }

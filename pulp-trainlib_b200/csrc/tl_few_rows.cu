@@ -7,7 +7,8 @@
 //   What counts is the number of loads under way: a thread issues all of a turn's, 256 bytes of weights, before it waits for the first.
 //   (Rings in shared memory with even shares of all bytes for persistent CTAs, by bulk copies of 1 KB or by cp.async, keep more under way, but lose more than
 //   that at the ends of the units: 8-bit 4096 -> 10240 for one token 16 us against 11, fp16 4096 x 10240 x 4096 57 us against 54.)
-//   Rows that do not start on 16 bytes come as the five words around the thread's bytes, shifted into place.
+//   Rows that do not start on 16 bytes come as the five words around the thread's bytes, shifted into place, without a condition up to the last piece or two of
+//   a row (23 tokens of 1000 x 2731 x 1000: 15.7 us; a condition around every piece's words, each waiting for the one before, 18.8; 2736: 11.0).
 //   Half precision, up to eight tokens: silu(gate) * up goes from one product to the other in two halves, itself and what its rounding left: the weights' bytes
 //   are what counts, and the result is rounded once (one token of 4096 x 10240 x 4096: 45.9 us, with one rounded half 44.4; 32 tokens would take 76 for 66).
 //   Single precision: the same on m16n8k8 in TF32, every operand as two parts and three products of them; the sums move to others, rounded to nearest, after
@@ -15,6 +16,7 @@
 #include "tl_gate.cuh"
 #include "tl_tc.cuh"
 #include "tl_reduce.cuh"
+#include <type_traits>
 
 namespace tl {
 
@@ -29,6 +31,7 @@ template <class T> struct FewParams {
     const T *bias; const float *xs, *ws;
     int rows, M, K;                     // tokens, weight rows, elements of K
     long long x_stride, c_stride;       // elements
+    bool words, x16;                    // every tensor starts on four bytes; x's rows on sixteen
 };
 
 // 16 neighbouring bytes of a row of K elements from element k on, zeros behind the end.  ALIGN < 16: rows start anywhere.  Inside a row (four bytes in front of the
@@ -67,6 +70,32 @@ __device__ __forceinline__ uint4 few_keep(const void *p)
     uint4 v;
     asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
+}
+__device__ __forceinline__ uint32_t few_word(const void *p)
+{
+    uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+// 16 bytes of a row that starts on four bytes or between: the five words around them as they come, to be shifted into place when they are used
+struct FewRaw { uint32_t w[5]; };
+template <class E> __device__ __forceinline__ FewRaw few_raw(const E *at, bool whole)
+{
+    FewRaw r;
+    if (whole) {                                             // (the row starts on sixteen)
+        const uint4 v = few_keep(at);
+        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w; r.w[4] = 0;
+    } else {
+        const uint32_t *from = reinterpret_cast<const uint32_t *>((uintptr_t)at & ~(uintptr_t)3);
+#pragma unroll
+        for (int i = 0; i < 5; i++) r.w[i] = few_word(from + i);
+    }
+    return r;
+}
+__device__ __forceinline__ uint4 few_place(const FewRaw &r, const void *row)
+{
+    const uint32_t sh = (uint32_t)((uintptr_t)row & 3) * 8u;                 // (pieces are multiples of four bytes)
+    return make_uint4(__funnelshift_r(r.w[0], r.w[1], sh), __funnelshift_r(r.w[1], r.w[2], sh), __funnelshift_r(r.w[2], r.w[3], sh), __funnelshift_r(r.w[3], r.w[4], sh));
 }
 __device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
@@ -176,6 +205,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
         }
     };
     int k0 = 0;
+    constexpr int UT = ALIGN == 16 ? 1 : MT * MATS == 1 ? 4 : 2;
     if constexpr (ALIGN == 16) {
         for (; k0 + WARPS * PIECE * U <= p.K; k0 += WARPS * PIECE * U) {
             uint4 wv[U][MATS][MT][2], xv[U][XP * NT];
@@ -197,8 +227,46 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
             for (int i = 0; i < U; i++) multiply(wv[i], xv[i]);
             settle();
         }
+    } else if (p.words && p.K > WARPS * PIECE * (F32 ? UT : 1)) {             // (shorter rows: the loop below has them under way at once)
+        constexpr int WORD = 4 / (int)sizeof(E);             // (the fifth word of a piece is the row's too)
+        const int last = p.K - PIECE - WORD;                 // where a piece may start at most; what lies behind is left to the loop below
+        auto turn = [&](auto part) {
+            constexpr bool PART = decltype(part)::value;
+            FewRaw wr[U][MATS][MT][2], xr[U][XP * NT];
+            const int first = k0 + warp * PIECE;
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                if (PART && first + i * WARPS * PIECE > last) continue;
+                const int k = first + i * WARPS * PIECE + t * N;
+#pragma unroll
+                for (int b = 0; b < MATS; b++)
+#pragma unroll
+                    for (int a = 0; a < MT; a++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) wr[i][b][a][h] = few_raw(wp[b][a][h] + k, false);
+#pragma unroll
+                for (int n = 0; n < XP * NT; n++) xr[i][n] = few_raw(xp[n % NT] + (n < NT ? 0 : rest) + k, p.x16);
+            }
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                if (PART && first + i * WARPS * PIECE > last) continue;
+                uint4 wv[MATS][MT][2], xv[XP * NT];
+#pragma unroll
+                for (int b = 0; b < MATS; b++)
+#pragma unroll
+                    for (int a = 0; a < MT; a++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) wv[b][a][h] = few_place(wr[i][b][a][h], wp[b][a][h]);
+#pragma unroll
+                for (int n = 0; n < XP * NT; n++) xv[n] = few_place(xr[i][n], xp[n % NT] + (n < NT ? 0 : rest));
+                multiply(wv, xv);
+            }
+            settle();
+        };
+        for (; k0 + (WARPS * U - 1) * PIECE <= last; k0 += WARPS * PIECE * U) turn(std::false_type{});
+        if (k0 <= last) turn(std::true_type{});
+        k0 = last < 0 ? 0 : (last / PIECE + 1) * PIECE;      // the one or two pieces behind
     }
-    constexpr int UT = ALIGN == 16 ? 1 : MT * MATS == 1 ? 4 : 2;
     for (; k0 < p.K; k0 += WARPS * PIECE * UT) {
         uint4 wv[UT][MATS][MT][2], xv[UT][XP * NT];
 #pragma unroll
@@ -313,8 +381,11 @@ template <int KIND, class T, int EPI, int ALIGN> static void few_tokens(const Fe
 template <int KIND, class T, int EPI> static void few_aligned(const FewParams<T> &p, int esize)
 {
     const uintptr_t at = (uintptr_t)p.x | (uintptr_t)p.x2 | (uintptr_t)p.w[0] | (uintptr_t)(EPI == FFN_GATE ? p.w[1] : nullptr) | (uintptr_t)((long long)p.K * esize) | (uintptr_t)(p.x_stride * esize);
-    if (at % 16 == 0) few_tokens<KIND, T, EPI, 16>(p);
-    else few_tokens<KIND, T, EPI, 1>(p);
+    if (at % 16 == 0) return few_tokens<KIND, T, EPI, 16>(p);
+    FewParams<T> q = p;
+    q.words = (((uintptr_t)p.x | (uintptr_t)p.x2 | (uintptr_t)p.w[0] | (uintptr_t)(EPI == FFN_GATE ? p.w[1] : nullptr)) & 3) == 0;
+    q.x16 = (((uintptr_t)p.x | (uintptr_t)p.x2 | (uintptr_t)(p.x_stride * esize)) & 15) == 0;
+    few_tokens<KIND, T, EPI, 1>(q);
 }
 template <int EPI> static void few_fp32(const FewParams<float> &p)
 {

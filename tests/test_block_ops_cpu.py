@@ -62,6 +62,13 @@ def test_sums_that_pass_32_bits_are_refused(p):
     assert outcome("trainlib_linear_int8_%s_fw_cl" % p, "trainlib_linear_int8_args", {**LIN8, "in_size": 131072}) == (TOO_LARGE, True)
 
 
+@pytest.mark.parametrize("size", ["rows", "in_size", "hidden", "out_size"])
+@pytest.mark.parametrize("p", ["fp32", "fp16"])
+def test_sizes_beyond_the_index_arithmetic_are_refused(p, size):
+    for name, fields in (("trainlib_gated_ffn_%s_fw_cl", FFN), ("trainlib_gated_ffn_%s_bw_cl", FFN_BW)):
+        assert outcome(name % p, "trainlib_gated_ffn_args", {**fields, size: (1 << 30) + 1}) == (TOO_LARGE, True)
+
+
 def test_null_arguments_and_a_machine_without_a_device(pkg):
     lib = pkg.load()
     for name in pkg.EXT_FUNCTIONS:

@@ -407,6 +407,33 @@ def test_ffn_of_many_tiles(ops, rows, n, h, m):
 
 
 @both
+@pytest.mark.parametrize("rows", [1, 9, 20, 32])
+def test_ffn_few_tokens_of_odd_widths(ops, rows, dt):
+    """rows that start between two groups of sixteen bytes and end around a whole number of what the warps take at a time, in the first products and in the last"""
+    for k in (127, 131, 257, 511, 513, 545, 1025, 1027, 2050, 2731):
+        for n, h in ((k, 24), (40, k)):
+            for shift in (0, 2):
+                x, wg, wu, wd = ffn_tensors(rows, n, h, 33, dt, shift, seed=50 + k)
+                gd, ud = x.double() @ wg.double().T, x.double() @ wu.double().T
+                y = blank(rows, 33, dt=dt)
+                ops.ffn_fw(x, wg, wu, wd, None, None, y)
+                near(y, (silu(gd) * ud) @ wd.double().T, dt, 2, (3 * n, h), "y", (silu(gd) * ud).square() @ wd.double().square().T)
+
+
+@pytest.mark.parametrize("rows", [1, 9, 20, 32, 33, 150])
+def test_linear_in_8_bits_of_odd_widths(ops, rows):
+    """whole numbers: the sums are exact and rounded once"""
+    gen = torch.Generator("cuda").manual_seed(rows)
+    for k in (515, 1023, 1025, 1026, 1087, 1089, 2113, 4099):
+        for shift in (0, 1, 4):
+            x = blank(rows, k, dt=torch.int8, shift=shift).copy_(torch.randint(-128, 128, (rows, k), device="cuda", generator=gen))
+            w = blank(37, k, dt=torch.int8, shift=shift).copy_(torch.randint(-128, 128, (37, k), device="cuda", generator=gen))
+            y = blank(rows, 37)
+            ops.linear_int8(x, torch.ones(rows, device="cuda"), w, torch.ones(37, device="cuda"), None, y)
+            assert torch.equal(y, (x.double() @ w.double().T).float()), (k, shift)
+
+
+@both
 def test_ffn_rows_of_no_numbers_stay_apart(ops, dt):
     for rows, n, h, m in ((3, 64, 96, 40), (200, 256, 384, 128), (300, 100, 70, 50)):
         x, wg, wu, wd = ffn_tensors(rows, n, h, m, dt)
