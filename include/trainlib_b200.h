@@ -142,7 +142,7 @@ void  trainlib_rmsnorm_fp16_bw_cl(void *trainlib_rmsnorm_args);
  *        dw_up; w_gate and w_up for dx; x for dw_gate and dw_up.  Any of dx, dw_gate, dw_up, dw_down may be NULL (not wanted), not all.
  * The product silu(gate) * up and its gradients are library scratch of `rows * hidden` elements each (`hidden` rounded up to 128
  * bytes): three of them in the backward pass; beside them copies of operands whose rows do not start on 16 bytes, in fp32 of every
- * operand twice, and partial sums of up to 64 MB.  In fp16 silu(gate) * up and the gradients are rounded to fp16 between the products
+ * operand twice, and partial sums of up to 64 MB a gradient.  In fp16 silu(gate) * up and the gradients are rounded to fp16 between the products
  * (what passes 65504 there is infinite); up to eight rows of a forward pass it goes on unrounded.  A call repeated gives the same bits;
  * rows, alignment and which gradients are asked for together may change the order of a sum.  Outputs must not overlap inputs.  A size
  * above 2^30 is refused (TL_ERR_TOO_LARGE). */
