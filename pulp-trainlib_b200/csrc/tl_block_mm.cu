@@ -73,6 +73,13 @@ template <int KIND, bool PAIR, int SA, int SB> __device__ __forceinline__ void b
     bm_mma<KIND, PAIR, SA, SB, 2>(d, a, b, idesc, acc);
     bm_mma<KIND, PAIR, SA, SB, 3>(d, a, b, idesc, acc);
 }
+// has the phase completed? (asked without waiting: mbarrier.try_wait may suspend the thread, for a stage that is not coming too)
+__device__ __forceinline__ bool bm_peek(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 // accumulators of 32-bit integers (2), operands of signed 8 bits (1), both K-major
 __host__ __device__ constexpr uint32_t i8_idesc(uint32_t M, uint32_t N) { return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24); }
 
@@ -442,7 +449,7 @@ __global__ void __launch_bounds__(BM_THREADS) block_mm_kernel(const __grid_const
                         if (!ready && !tm_wait(&full[s], phase, failed)) { ok = false; break; }
                         const int now = s;
                         if (++s == ST) { s = 0; phase ^= 1u; }
-                        ready = mbar_try_wait(&full[s], phase);                 // of the next step: its answer comes while this one's MMAs are issued
+                        ready = bm_peek(&full[s], phase);                       // of the next step: its answer comes while this one's MMAs are issued
                         tc_fence_after();
                         const uint32_t a = low_a + now * stage_step, b = low_b + now * stage_step;
                         if (KIND != MM_F16 || !(a_mn || b_mn)) bm_step<KIND, PAIR, 2, 2>(d, a, b, idesc, acc);
