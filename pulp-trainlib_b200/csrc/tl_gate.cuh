@@ -4,11 +4,17 @@
 
 namespace tl {
 
-// s = 1 / (1 + exp(-g)).  For half-precision results the hardware's exponential and quotient do (their few units of 2^-23, growing with |g| to some
-// thirty at the |g| where s is no longer 0 or 1 to eleven bits); both ends of the range are right: exp(-g) = inf gives 0.
+// s = 1 / (1 + exp(-g)).  For half-precision results the hardware's power of two and reciprocal do (their few units of 2^-23, growing with |g| to some
+// thirty at the |g| where s is no longer 0 or 1 to eleven bits), without subnormal numbers, which are nothing beside 1 and in a result of half precision;
+// both ends of the range are right: exp(-g) = inf gives 0.
 template <bool FAST> __device__ __forceinline__ float gate_sigmoid(float g)
 {
-    if constexpr (FAST) return __fdividef(1.f, 1.f + __expf(-g));
+    if constexpr (FAST) {
+        float e, s;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+        return s;
+    }
     else return 1.f / (1.f + expf(-g));
 }
 template <bool FAST> __device__ __forceinline__ float gate_fw(float g, float u) { return g * gate_sigmoid<FAST>(g) * u; }
