@@ -587,7 +587,7 @@ def test_host_tensors(ops, dt):
 
 
 @both
-@pytest.mark.parametrize("rows,n,h", [(3, 64, 96), (40, 512, 200), (300, 512, 640)])
+@pytest.mark.parametrize("rows,n,h", [(3, 64, 96), (40, 512, 200), (300, 512, 640), (20, 333, 777), (150, 259, 1001)])
 def test_recorded_and_replayed(ops, rows, n, h, dt):
     """two recorded graphs that share the library's scratch, replayed in turn on new inputs: the bits of direct calls"""
     def program(seed):
