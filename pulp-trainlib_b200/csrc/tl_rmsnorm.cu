@@ -790,6 +790,7 @@ template <class T> void rmsnorm_bw(Scope &sc, const T *h, const T *w, const T *d
     do {                                                                       \
         if (size <= 32 * V) TL_NORM_BW(32, 1, V, true);                        \
         else if (size <= 32 * E) TL_NORM_BW(32, E / V, V, true);               \
+        else if (size <= 64 * E) TL_NORM_BW(64, E / V, V, true);               \
         else if (size <= 128 * E) TL_NORM_BW(128, E / V, V, true);             \
         else if (size <= 256 * E) TL_NORM_BW(256, E / V, V, true);             \
         else if (size <= 512 * E) TL_NORM_BW(512, E / V, V, true);             \

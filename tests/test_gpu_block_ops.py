@@ -145,7 +145,7 @@ def test_norm_in_8_bits(ops, rows, size, shift, dt):
 
 
 @both
-@pytest.mark.parametrize("rows,size", NORMS + [(2000, 40), (4100, 512), (513, 2176)])
+@pytest.mark.parametrize("rows,size", NORMS + [(2000, 40), (4100, 512), (513, 2176), (700, 331), (1300, 499), (40, 510)])
 def test_norm_backward(ops, rows, size, dt):
     for shift in (0, 1):
         h, dy, dsum = randn(7, rows, size, scale=2, dt=dt, shift=shift), randn(8, rows, size, dt=dt, shift=shift), randn(9, rows, size, dt=dt, shift=shift)
