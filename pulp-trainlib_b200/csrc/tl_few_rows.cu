@@ -8,7 +8,7 @@
 //   (Rings in shared memory with even shares of all bytes for persistent CTAs, by bulk copies of 1 KB or by cp.async, keep more under way, but lose more than
 //   that at the ends of the units: 8-bit 4096 -> 10240 for one token 16 us against 11, fp16 4096 x 10240 x 4096 57 us against 54.)
 //   Rows that do not start on 16 bytes come as the five words around the thread's bytes, shifted into place, without a condition up to the last piece or two of
-//   a row (23 tokens of 1000 x 2731 x 1000: 15.7 us; a condition around every piece's words, each waiting for the one before, 18.8; 2736: 11.0).
+//   a row (23 tokens of 1000 x 2731 x 1000: 15.7 us; a condition around every piece's words, each waiting for the one before, 18.8; 2736: 10.5).
 //   Half precision, up to eight tokens: silu(gate) * up goes from one product to the other in two halves, itself and what its rounding left: the weights' bytes
 //   are what counts, and the result is rounded once (one token of 4096 x 10240 x 4096: 45.9 us, with one rounded half 44.4; 32 tokens would take 76 for 66).
 //   Single precision: the same on m16n8k8 in TF32, every operand as two parts and three products of them; the sums move to others, rounded to nearest, after
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
         }
     };
     int k0 = 0;
-    constexpr int UT = ALIGN == 16 ? 1 : MT * MATS == 1 ? 4 : 2;
+    constexpr int UT = ALIGN == 16 ? KIND != FEW_F16 ? 1 : MT * MATS == 1 ? U : 2 : MT * MATS == 1 ? 4 : 2;        // (pieces under way where a row ends)
     if constexpr (ALIGN == 16) {
         for (; k0 + WARPS * PIECE * U <= p.K; k0 += WARPS * PIECE * U) {
             uint4 wv[U][MATS][MT][2], xv[U][XP * NT];
