@@ -865,7 +865,7 @@ template <class T> void linear_int8(Scope &sc, const signed char *x, const float
 {
     if (rows <= FEW_ROWS) return few_rows_int8<T>(sc, x, xs, w, ws, bias, y, rows, in, out);
     if (!bm_ready()) return;
-    const int quads = ceil_div(in, 128) * 8;                 // (whole lines, as above)
+    const int quads = in < 128 ? ceil_div(in, 16) : ceil_div(in, 128) * 8;         // (whole lines, as above, where a row has one)
     const signed char *at[2] = {x, w};
     signed char *copy[2] = {nullptr, nullptr};
     const int count[2] = {rows, out};
