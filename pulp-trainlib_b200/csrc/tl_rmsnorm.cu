@@ -24,10 +24,11 @@ __device__ __forceinline__ float2 quant_factor(float m)
 }
 // v / (m / 127) to the nearest whole number, V values at a time into bytes.  Adding 1.5 * 2^23 leaves the nearest whole number (ties to even) in the low bits.
 // The quotient in 32 bits is off by three roundings, 127 * 3 * 2^-24 at most: where one of the values lies that near the border of two steps (a few
-// in a hundred thousand, and every exact tie), and in rows that are not finite, 64 bits decide.
+// in a hundred thousand, and every exact tie), and in rows that are not finite, 64 bits decide: 127 v is exact there (31 bits), so the one rounding of the
+// quotient leaves a tie a tie.  (A rounded m / 127 as the divisor put half of a row's largest magnitude, 63.5 steps, at 63 for an eighth of all m.)
 __device__ __noinline__ int quant_exact(float v, float m)
 {
-    const double n = rint((double)v / ((double)m / 127.0));
+    const double n = rint((double)v * 127.0 / (double)m);
     return m > 0.f && n == n ? (int)fmin(fmax(n, -127.0), 127.0) : 0;
 }
 template <int V> __device__ __forceinline__ void quant(const float (&v)[V], float2 f, float m, bool finite, signed char (&q)[V])

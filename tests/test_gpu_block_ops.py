@@ -689,3 +689,30 @@ def test_the_same_bits_every_time_and_nothing_beside_them(ops, dt):
             now = [v.clone() for v in t.values()] + [q, s]
             assert first is None or all(torch.equal(a, b) for a, b in zip(first, now))
             first = now
+
+
+@both
+@pytest.mark.parametrize("size", [40, 300, 1001, 4096, 40000])
+def test_ties_between_two_steps_go_to_the_even_one(ops, size, dt):
+    """values that lie in the middle of two steps: half of a row's largest magnitude (63.5 steps), and in rows whose largest magnitude is 127 times a
+    power of two every half step.  Whole numbers: the same ones from the rows, and from the norm with weights of one (its h times 1 is rounded nowhere)."""
+    rows = 64
+    x = randn(120, rows, size, dt=dt).clamp(-4, 4)
+    top = (4 + randn(121, rows).abs()).to(dt)                            # (a half of them is a number of either type, too)
+    x[:, 0], x[:, 3], x[:, size - 1] = top, top / 2, -top / 2
+    want = torch.round(x.double() * 127 / top.double()[:, None])         # 127 x is exact in 64 bits, and the quotient of a tie a whole number and a half
+    assert (want[:, 3] == 64).all() and (want[:, size - 1] == -64).all()
+    steps = torch.arange(size, device="cuda") % 254 - 126.5
+    power = 2.0 ** (torch.arange(rows, device="cuda") % 9 - 4)
+    y = (steps[None, :] * power[:, None]).to(dt)
+    y[:, 1] = (127 * power).to(dt)
+    even = torch.round(steps.double())[None, :].repeat(rows, 1)
+    even[:, 1] = 127
+    q, scale, ones = blank(rows, size, dt=torch.int8), blank(rows), torch.ones(size, device="cuda", dtype=dt)
+    for shift in (0, 1):
+        for v, whole in ((x, want), (y, even)):
+            room = blank(rows, size, dt=dt, shift=shift).copy_(v)
+            ops.rows_int8(room, q, scale)
+            assert torch.equal(q.double(), whole)
+            ops.norm_int8(room, None, ones, None, q, scale)
+            assert torch.equal(q.double(), whole)
