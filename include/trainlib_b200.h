@@ -114,7 +114,7 @@ void  trainlib_gelu_fp16_bw_cl(void *act_args_fp16);
  *          sum, if not NULL, receives h.  sum or output may be x or residual itself.
  *   int8:  the same, rounded to 8 bits with a scale for each row: q * scale = weight * h / sqrt(mean(h^2) + eps), scale = the row's
  *          largest magnitude / 127, q rounded to nearest (ties to even).  A row of zeros has scale 0; a row whose result is not
- *          finite has a scale that is not finite (q is 0 where a value is NaN).
+ *          finite (or whose products weight * h are not) has a scale that is not finite (q is 0 where a value is NaN).
  *   bw:    `sum` is the input: the h that the forward pass left.  With r = 1 / sqrt(mean(h^2) + eps) and g = weight * dy:
  *          dx = dsum + r * (g - h * r^2 * mean(g * h)) is the gradient of x and of residual; dsum (NULL: none) is the gradient that
  *          reaches the sum along the residual path.  dweight[j] = sum over the rows of dy * h * r.  dx or dweight may be NULL (not

@@ -51,7 +51,7 @@ template <int V> __device__ __forceinline__ void quant(const float (&v)[V], floa
 #pragma unroll
     for (int i = 0; i < V; i++) q[i] = (signed char)(u[i] & 255u);
 }
-// a row's scale from r, its largest magnitude and a sum that is finite if all of it is
+// a row's scale from r, its largest magnitude and a sum that is finite if all of it is (of h^2 and, for the norm, 0 * w h: NaN where w h is no finite number)
 __device__ __forceinline__ float quant_scale(float r, float m, float sum) { return sum - sum == 0.f ? r * __fdiv_rn(m, 127.f) : sum * 0.f; }
 
 // 1 / sqrt(v): the hardware's value (off by 2^-22.9) and one step of Newton's method; v = inf gives 0
@@ -432,7 +432,11 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, fw_blocks(G, NV, MODE == QU
             for (int e = 0; e < P; e++) {
                 h[k][e] = add2(h[k][e], c[e]);
                 s2 = fma2(h[k][e], MODE == QUANT_ROWS ? twice(0.f) : h[k][e], s2);       // (quantised alone, the sum tells only whether every value is finite)
-                if (MODE != NORM_PLAIN) { const float2 v = MODE == NORM_INT8 ? mul2(h[k][e], ww[e]) : h[k][e]; m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))); }
+                if (MODE != NORM_PLAIN) {
+                    const float2 v = MODE == NORM_INT8 ? mul2(h[k][e], ww[e]) : h[k][e];
+                    m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y)));
+                    if (MODE == NORM_INT8) s2 = fma2(v, twice(0.f), s2);                  // (a weight that is no number shows in the sum, too)
+                }
             }
         }
         const float2 tot = row_reduce<G, true>(s2.x + s2.y, m, red);     // (the largest magnitude passes over NaN: the scale carries it)
@@ -463,7 +467,11 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, fw_blocks(G, NV, MODE == QU
         for (int i = 0; i < V; i++) {
             h[k][i] = tof(a[k].e[i]) + tof(b[k].e[i]);
             s = MODE == QUANT_ROWS ? fmaf(h[k][i], 0.f, s) : fmaf(h[k][i], h[k][i], s);                  // (quantised alone, the sum tells only whether every value is finite)
-            if (MODE != NORM_PLAIN) m = fmaxf(m, fabsf(MODE == NORM_INT8 ? h[k][i] * tof(wv[k].e[i]) : h[k][i]));       // (passes over NaN: the scale carries it)
+            if (MODE != NORM_PLAIN) {
+                const float v = MODE == NORM_INT8 ? h[k][i] * tof(wv[k].e[i]) : h[k][i];
+                m = fmaxf(m, fabsf(v));                                                                  // (passes over NaN: the scale carries it)
+                if (MODE == NORM_INT8) s = fmaf(v, 0.f, s);                                              // (and a weight's that is none)
+            }
         }
     const float2 tot = row_reduce<G, true>(s, m, red);
     if (row >= rows) return;
@@ -490,7 +498,11 @@ __global__ void __launch_bounds__(1024) rmsnorm_fw_wide_kernel(const T *x, const
     for (int j = threadIdx.x; j < size; j += 1024) {
         const float h = ld(x + at + j) + (res ? ld(res + at + j) : 0.f);
         s = MODE == QUANT_ROWS ? fmaf(h, 0.f, s) : fmaf(h, h, s);
-        if (MODE != NORM_PLAIN) m = fmaxf(m, fabsf(MODE == NORM_INT8 ? h * ld(w + j) : h));
+        if (MODE != NORM_PLAIN) {
+            const float v = MODE == NORM_INT8 ? h * ld(w + j) : h;
+            m = fmaxf(m, fabsf(v));
+            if (MODE == NORM_INT8) s = fmaf(v, 0.f, s);
+        }
     }
     const float2 tot = row_reduce<1024, true>(s, m, red);
     const float r = MODE == QUANT_ROWS ? 1.f : norm_factor(fmaf(tot.x, per, eps));

@@ -716,3 +716,27 @@ def test_ties_between_two_steps_go_to_the_even_one(ops, size, dt):
             assert torch.equal(q.double(), whole)
             ops.norm_int8(room, None, ones, None, q, scale)
             assert torch.equal(q.double(), whole)
+
+
+@both
+@pytest.mark.parametrize("size", [5, 34, 96, 1000, 1001, 4096, 16384, 40000])
+def test_norm_weights_that_are_no_numbers(ops, size, dt):
+    """a weight that is NaN or infinite is part of every row: in 8 bits no row has a finite scale, and q is 0 in the NaN's column; also where
+    every other value of the row is zero.  The sum that goes on along the residual path keeps its bits."""
+    rows = 5
+    x, res = randn(130, rows, size, dt=dt), randn(131, rows, size, dt=dt)
+    x[1], res[1] = 0, 0
+    w = (1 + randn(132, size, scale=0.3)).to(dt)
+    clean = blank(rows, size, dt=dt)
+    ops.norm_fw(x, res, w, clean, blank(rows, size, dt=dt))
+    for shift in (0, 1):
+        a, b = blank(rows, size, dt=dt, shift=shift).copy_(x), blank(rows, size, dt=dt, shift=shift).copy_(res)
+        for what in (float("nan"), float("inf"), -float("inf")):
+            for at in (0, size // 2, size - 1):
+                bad = w.clone()
+                bad[at] = what
+                total, q, scale = blank(rows, size, dt=dt, shift=shift), blank(rows, size, dt=torch.int8, shift=shift), blank(rows)
+                ops.norm_int8(a, b, bad, total, q, scale)
+                assert not torch.isfinite(scale).any(), (what, at)
+                assert (q[:, at] == 0).all(), (what, at)
+                assert torch.equal(total, clean)
