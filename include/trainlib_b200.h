@@ -107,7 +107,7 @@ void  trainlib_gelu_fp16_bw_cl(void *act_args_fp16);
  * the matrix product [ref: lib/sources/pulp_rmsnorm_fp32.c:29-60, lib/sources/pulp_act_fp32.c:688-712].  Tensors are row-major and dense, a row per token; T is
  * float for the fp32 entry points and fp16 for the fp16 ones.  Sums, statistics and scales are held in 32 bits.  The streams mode
  * does not apply: `rows` counts every token.  Calls with rows or a size below 1, or without a pointer that they need, are refused
- * (TL_ERR_BAD_ARGS) and touch nothing.  Host pointers are staged like everywhere; gradients are written, not accumulated.
+ * (TL_ERR_BAD_ARGS), as are rows or sizes above 2^30 (TL_ERR_TOO_LARGE), and touch nothing.  Host pointers are staged like everywhere; gradients are written, not accumulated.
  *
  * RMS norm of a residual sum.
  *   fw:    h = x + residual (residual may be NULL: h = x);  output = weight * h / sqrt(mean(h^2) + eps) from the unrounded h;
@@ -144,8 +144,8 @@ void  trainlib_rmsnorm_fp16_bw_cl(void *trainlib_rmsnorm_args);
  * bytes): three of them in the backward pass; beside them copies of operands whose rows do not start on 16 bytes, in fp32 of every
  * operand twice, and partial sums of up to 64 MB a gradient.  In fp16 silu(gate) * up and the gradients are rounded to fp16 between the products
  * (what passes 65504 there is infinite); up to eight rows of a forward pass it goes on unrounded.  A call repeated gives the same bits;
- * rows, alignment and which gradients are asked for together may change the order of a sum.  Outputs must not overlap inputs.  A size
- * above 2^30 is refused (TL_ERR_TOO_LARGE). */
+ * rows, alignment and which gradients are asked for together may change the order of a sum.  Outputs must not overlap inputs or
+ * each other. */
 struct trainlib_gated_ffn_args {
     void *x; void *w_gate; void *w_up; void *w_down; void *gate; void *up; void *y;
     int rows; int in_size; int hidden; int out_size;

@@ -10,11 +10,21 @@ namespace {
 #define TL_REQUIRE(cond, ...)                                        \
     do { if (!(cond)) { set_error(TL_ERR_BAD_ARGS, __VA_ARGS__); return; } } while (0)
 
+// The kernels' indices are 32 bits wide and run up to a few thousand beyond a size.
+bool sizes_fit(const char *what, int a, int b)
+{
+    const int largest = std::max(a, b);
+    if (largest <= 1 << 30) return true;
+    set_error(TL_ERR_TOO_LARGE, "%s: a size of %d, 2^30 at most", what, largest);
+    return false;
+}
+
 template <class T> void rmsnorm_fw_impl(void *args, bool int8)
 {
     auto *a = (trainlib_rmsnorm_args *)args;
     TL_REQUIRE(a && a->rows > 0 && a->size > 0, "trainlib_rmsnorm: rows=%d size=%d", a ? a->rows : 0, a ? a->size : 0);
     TL_REQUIRE(a->x && a->weight && (int8 ? a->q && a->scale : a->output != nullptr), "trainlib_rmsnorm: null x, weight or output");
+    if (!sizes_fit("trainlib_rmsnorm", a->rows, a->size)) return;
     Scope sc;
     const size_t n = (size_t)a->rows * a->size;
     const T *x = sc.in((T *)a->x, n), *res = sc.in((T *)a->residual, n), *w = sc.in((T *)a->weight, (size_t)a->size);
@@ -33,6 +43,7 @@ template <class T> void rmsnorm_bw_impl(void *args)
     auto *a = (trainlib_rmsnorm_args *)args;
     TL_REQUIRE(a && a->rows > 0 && a->size > 0, "trainlib_rmsnorm: rows=%d size=%d", a ? a->rows : 0, a ? a->size : 0);
     TL_REQUIRE(a->sum && a->weight && a->dy && (a->dx || a->dweight), "trainlib_rmsnorm: backward needs sum, weight, dy and a gradient to write");
+    if (!sizes_fit("trainlib_rmsnorm", a->rows, a->size)) return;
     Scope sc;
     const size_t n = (size_t)a->rows * a->size;
     const T *h = sc.in((T *)a->sum, n), *w = sc.in((T *)a->weight, (size_t)a->size), *dy = sc.in((T *)a->dy, n), *dsum = sc.in((T *)a->dsum, n);
@@ -45,6 +56,7 @@ template <class T> void quantize_rows_impl(void *args)
 {
     auto *a = (trainlib_quantize_rows_args *)args;
     TL_REQUIRE(a && a->rows > 0 && a->size > 0 && a->x && a->q && a->scale, "trainlib_quantize_rows: rows=%d size=%d or a null pointer", a ? a->rows : 0, a ? a->size : 0);
+    if (!sizes_fit("trainlib_quantize_rows", a->rows, a->size)) return;
     Scope sc;
     const size_t n = (size_t)a->rows * a->size;
     const T *x = sc.in((T *)a->x, n);
@@ -57,6 +69,7 @@ template <class T> void linear_int8_impl(void *args)
     auto *a = (trainlib_linear_int8_args *)args;
     TL_REQUIRE(a && a->rows > 0 && a->in_size > 0 && a->out_size > 0, "trainlib_linear_int8: rows=%d in_size=%d out_size=%d", a ? a->rows : 0, a ? a->in_size : 0, a ? a->out_size : 0);
     TL_REQUIRE(a->x && a->x_scale && a->weight && a->w_scale && a->y, "trainlib_linear_int8: null operand, scale or output");
+    if (!sizes_fit("trainlib_linear_int8", a->rows, a->out_size)) return;
     if (a->in_size > 131071) { set_error(TL_ERR_TOO_LARGE, "trainlib_linear_int8: in_size = %d, sums of more than 131071 products pass 32 bits", a->in_size); return; }
     Scope sc;
     const signed char *x = sc.in(a->x, (size_t)a->rows * a->in_size), *w = sc.in(a->weight, (size_t)a->out_size * a->in_size);
@@ -68,10 +81,7 @@ template <class T> void linear_int8_impl(void *args)
 template <class T> bool gated_ffn_sizes(trainlib_gated_ffn_args *a)
 {
     if (a && a->rows > 0 && a->in_size > 0 && a->hidden > 0 && a->out_size > 0) {
-        const int largest = std::max(std::max(a->rows, a->in_size), std::max(a->hidden, a->out_size));
-        if (largest <= 1 << 30) return true;
-        set_error(TL_ERR_TOO_LARGE, "trainlib_gated_ffn: a size of %d, 2^30 at most", largest);
-        return false;
+        return sizes_fit("trainlib_gated_ffn", std::max(a->rows, a->in_size), std::max(a->hidden, a->out_size));
     }
     set_error(TL_ERR_BAD_ARGS, "trainlib_gated_ffn: rows=%d in_size=%d hidden=%d out_size=%d", a ? a->rows : 0, a ? a->in_size : 0, a ? a->hidden : 0, a ? a->out_size : 0);
     return false;

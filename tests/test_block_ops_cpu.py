@@ -80,3 +80,17 @@ def test_null_arguments_and_a_machine_without_a_device(pkg):
         for name, struct, fields in (("trainlib_rmsnorm_fp32_fw_cl", "trainlib_rmsnorm_args", NORM), ("trainlib_gated_ffn_fp32_bw_cl", "trainlib_gated_ffn_args", FFN_BW),
                                      ("trainlib_linear_int8_fp32_fw_cl", "trainlib_linear_int8_args", LIN8)):
             assert outcome(name, struct, fields) == (NO_DEVICE, True)
+
+
+LIMITS = [("trainlib_rmsnorm_%s_fw_cl", "trainlib_rmsnorm_args", NORM, ("rows", "size")), ("trainlib_rmsnorm_int8_%s_fw_cl", "trainlib_rmsnorm_args", NORM8, ("rows", "size")),
+          ("trainlib_rmsnorm_%s_bw_cl", "trainlib_rmsnorm_args", NORM_BW, ("rows", "size")), ("trainlib_quantize_rows_%s_cl", "trainlib_quantize_rows_args", ROWS8, ("rows", "size")),
+          ("trainlib_linear_int8_%s_fw_cl", "trainlib_linear_int8_args", LIN8, ("rows", "out_size"))]
+
+
+@pytest.mark.parametrize("p", ["fp32", "fp16"])
+@pytest.mark.parametrize("name,struct,fields,sizes", LIMITS, ids=[r[0][9:].replace("_%s", "").replace("_cl", "") for r in LIMITS])
+def test_sizes_that_wrap_around_are_refused(p, name, struct, fields, sizes):
+    """above 2^30 in every operator: a row's or a column's index plus what a pass adds to it stays below 2^31"""
+    for size in sizes:
+        for n in ((1 << 30) + 1, (1 << 31) - 1):
+            assert outcome(name % p, struct, {**fields, size: n}) == (TOO_LARGE, True), (size, n)
