@@ -729,7 +729,7 @@ template <int KIND, class T, int EPI> static bool bm_setup(Scope &sc, const BmPl
         if (j.splits > 1) p.reduce_blocks += j.tiles_m * j.tiles_n * (BM_ROWS * bnc / 4 / 256);
         if (j.splits > 1 && !(j.part = sc.scratch<uint32_t>((size_t)j.tiles_m * j.tiles_n * j.splits * BM_ROWS * plan.BN))) return false;
     }
-    return p.status != nullptr;
+    return true;
 }
 
 template <class T> static int bm_align(int ld, const void *a, const void *b, const void *c)
@@ -739,8 +739,9 @@ template <class T> static int bm_align(int ld, const void *a, const void *b, con
 }
 static bool bm_ready()
 {
-    if (tc_encode_tiled_fn()) return true;
-    set_error(TL_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    if (!tc_encode_tiled_fn()) set_error(TL_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    else if (!tc_status_word()) set_error(TL_ERR_NO_MEMORY, "no memory for the word in which a kernel's waits report");
+    else return true;
     return false;
 }
 static bool bm_no_map()

@@ -6,10 +6,13 @@
 
 static struct { char *p; size_t n; } blocks[256];
 static cudaError_t last = cudaSuccess;
-static int launches, fail_at, max_cluster, max_blocks, cluster_limit = 16;
+static int launches, fail_at, max_cluster, max_blocks, cluster_limit = 16, has_encoder;
+static size_t no_memory_for;
 
 void fake_reset(int fail) { launches = max_cluster = max_blocks = 0; fail_at = fail; }   /* fail: number of the launch that fails, from 1; 0: none */
 void fake_cluster_limit(int n) { cluster_limit = n; }
+void fake_encoder(int on) { has_encoder = on; }              /* the driver makes tensor maps (of nothing); asked for once by the library */
+void fake_no_memory_for(size_t n) { no_memory_for = n; }     /* device allocations of up to n bytes fail */
 int fake_launches(void) { return launches; }
 int fake_max_cluster(void) { return max_cluster; }
 int fake_max_blocks(void) { return max_blocks; }           /* of a launch, along x and y */
@@ -23,7 +26,7 @@ cudaError_t cudaGetDeviceProperties_v2(struct cudaDeviceProp *p, int d) { (void)
 cudaError_t cudaDeviceGetAttribute(int *v, enum cudaDeviceAttr a, int d) { (void)a; (void)d; *v = 148; return cudaSuccess; }
 cudaError_t cudaMalloc(void **p, size_t n)
 {
-    if (posix_memalign(p, 256, n)) return cudaErrorMemoryAllocation;
+    if (n <= no_memory_for || posix_memalign(p, 256, n)) return last = cudaErrorMemoryAllocation;
     memset(*p, 0x55, n);
     for (int i = 0; i < 256; i++) if (!blocks[i].p) { blocks[i].p = *p; blocks[i].n = n; break; }
     return cudaSuccess;
@@ -55,10 +58,11 @@ cudaError_t cudaEventCreate(cudaEvent_t *e) { *e = (cudaEvent_t)malloc(8); retur
 cudaError_t cudaEventCreateWithFlags(cudaEvent_t *e, unsigned f) { (void)f; return cudaEventCreate(e); }
 cudaError_t cudaEventRecord(cudaEvent_t e, cudaStream_t s) { (void)e; (void)s; return cudaSuccess; }
 cudaError_t cudaFuncSetAttribute(const void *f, enum cudaFuncAttribute a, int v) { (void)f; (void)a; (void)v; return cudaSuccess; }
+static int encode(void) { return 0; }
 cudaError_t cudaGetDriverEntryPoint(const char *s, void **p, unsigned long long f, enum cudaDriverEntryPointQueryResult *r)
 {
-    (void)s; (void)f; *p = NULL;
-    if (r) *r = cudaDriverEntryPointSymbolNotFound;
+    (void)s; (void)f; *p = has_encoder ? (void *)encode : NULL;
+    if (r) *r = has_encoder ? cudaDriverEntryPointSuccess : cudaDriverEntryPointSymbolNotFound;
     return cudaSuccess;
 }
 cudaError_t cudaOccupancyMaxActiveClusters(int *n, const void *f, const cudaLaunchConfig_t *c)

@@ -91,3 +91,25 @@ for half in ("", "_fp16"):
         most = max(most, fake.fake_max_cluster())
 assert most == %d, most
 """ % (limit, limit))
+
+
+def test_block_products_without_a_status_word_are_an_error(on_fake_runtime):
+    """the word in which a kernel's bounded wait reports cannot be allocated: products and 8-bit layers launch nothing and say so, and work once it can"""
+    on_fake_runtime(r"""
+fake.fake_encoder(1)
+x = lib.trainlib_malloc(1 << 22)
+keep = pkg.Keep()
+calls = []
+for p in ("fp32", "fp16"):
+    f = pkg.make_args(keep, "trainlib_gated_ffn_args", x=x, w_gate=x, w_up=x, w_down=x, gate=x, up=x, y=x, dy=x, dx=x, dw_gate=x, dw_up=x, dw_down=x, rows=64, in_size=64, hidden=64, out_size=64)
+    l = pkg.make_args(keep, "trainlib_linear_int8_args", x=x, x_scale=x, weight=x, w_scale=x, y=x, rows=64, in_size=64, out_size=64)
+    calls += [("trainlib_gated_ffn_%s_fw_cl" % p, f), ("trainlib_gated_ffn_%s_bw_cl" % p, f), ("trainlib_linear_int8_%s_fw_cl" % p, l)]
+for memory in (False, True):
+    fake.fake_no_memory_for(ctypes.c_size_t(0 if memory else 4))
+    for name, args in calls:
+        lib.trainlib_clear_error()
+        fake.fake_reset(0)
+        getattr(lib, name)(ctypes.byref(args))
+        err, n = lib.trainlib_last_error(), fake.fake_launches()
+        assert (err == pkg.TL_OK and n > 0) if memory else (err != pkg.TL_OK and n == 0), (memory, name, err, n)
+""")
