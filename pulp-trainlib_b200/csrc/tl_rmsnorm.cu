@@ -385,12 +385,8 @@ __global__ void __launch_bounds__(RING_TPB) rmsnorm_bw_ring_kernel(const T *h, c
         block_columns<T, G, NV, V, RG, RING_TPB>(a, part + (size_t)blockIdx.x * size, reinterpret_cast<float *>(ring_mem), size, t, mine);
     }
 }
-// stages per group, or 0: the rows are too long for two
-template <class T> static int ring_stages(int groups, int in, int size)
-{
-    const int n = RING_BYTES / (groups * in * size * (int)sizeof(T));
-    return n < 2 ? 0 : std::min(n, RING_MOST);
-}
+// stages per group (two at least: a group's rows are 96 KB at most for all of them together)
+template <class T> static int ring_stages(int groups, int in, int size) { return std::min(RING_BYTES / (groups * in * size * (int)sizeof(T)), RING_MOST); }
 
 // ---------------------------------------------------------------- forward
 // G threads per row, a block's rows side by side, NV packs of V elements per thread; small CTAs, so that one's loads cover the other's stores.  Measured with
@@ -769,17 +765,16 @@ template <class T> void rmsnorm_bw(Scope &sc, const T *h, const T *w, const T *d
     }
     if (wide && size <= 512 * 16) {
         int *status = tc_status_word();
+        if (!status) return set_error(TL_ERR_NO_MEMORY, "no memory for the word in which a kernel's waits report");
 #define TL_NORM_BW_RING(G, NV)                                                                                                                                        \
     do {                                                                                                                                                              \
-        const int stages = status ? ring_stages<T>(RING_TPB / G, 3, size) : 0, blocks = std::min(ceil_div(rows, RING_TPB / G), sm_count());                           \
-        if (!stages) break;                                                                                                                                           \
+        const int stages = ring_stages<T>(RING_TPB / G, 3, size), blocks = std::min(ceil_div(rows, RING_TPB / G), sm_count());                                        \
         float *part = dw ? sc.scratch<float>((size_t)blocks * size) : nullptr;                                                                                        \
         if (dw && !part) return;                                                                                                                                      \
         static bool set = false;                                                                                                                                      \
         if (!set) set = cudaFuncSetAttribute(rmsnorm_bw_ring_kernel<T, G, NV, V16>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES) == cudaSuccess;          \
         TL_LAUNCH((rmsnorm_bw_ring_kernel<T, G, NV, V16>), blocks, RING_TPB, RING_BYTES, h, w, dy, dsum, dx, part, rows, size, stages, eps, status);                  \
         if (dw) norm_columns<T>(part, dw, size, blocks);                                                                                                              \
-        return;                                                                                                                                                       \
     } while (0)
         constexpr int E = 16 / V16;
         if (size <= 32 * 8) TL_NORM_BW_RING(32, (E + 1) / 2);
@@ -789,6 +784,7 @@ template <class T> void rmsnorm_bw(Scope &sc, const T *h, const T *w, const T *d
         else if (size <= 256 * 16) TL_NORM_BW_RING(256, E);
         else TL_NORM_BW_RING(512, E);
 #undef TL_NORM_BW_RING
+        return;
     }
 #define TL_NORM_BW(G, NV, V, PRE)                                                                                                                             \
     do {                                                                                                                                                      \
@@ -799,20 +795,15 @@ template <class T> void rmsnorm_bw(Scope &sc, const T *h, const T *w, const T *d
         TL_LAUNCH((rmsnorm_bw_kernel<T, G, NV, V, PRE>), blocks, TPB, RG > 1 ? RG * size * sizeof(float) : 0, h, w, dy, dsum, dx, part, rows, size, eps);          \
         if (dw) norm_columns<T>(part, dw, size, blocks);                                                                                                      \
     } while (0)
-#define TL_NORM_BW_V(V, E)                                                     \
-    do {                                                                       \
-        if (size <= 32 * V) TL_NORM_BW(32, 1, V, true);                        \
-        else if (size <= 32 * E) TL_NORM_BW(32, E / V, V, true);               \
-        else if (size <= 64 * E) TL_NORM_BW(64, E / V, V, true);               \
-        else if (size <= 128 * E) TL_NORM_BW(128, E / V, V, true);             \
-        else if (size <= 256 * E) TL_NORM_BW(256, E / V, V, true);             \
-        else if (size <= 512 * E) TL_NORM_BW(512, E / V, V, true);             \
-        else if (size <= 1024 * 8) TL_NORM_BW(1024, 8 / V, V, false);          \
-        else TL_NORM_BW(1024, 16 / V, V, false);                               \
-    } while (0)
-    if (wide) TL_NORM_BW_V(V16, 2 * V16);
-    else TL_NORM_BW_V(1, 8);
-#undef TL_NORM_BW_V
+    if (wide) TL_NORM_BW(1024, 16 / V16, V16, false);
+    else if (size <= 32) TL_NORM_BW(32, 1, 1, true);
+    else if (size <= 32 * 8) TL_NORM_BW(32, 8, 1, true);
+    else if (size <= 64 * 8) TL_NORM_BW(64, 8, 1, true);
+    else if (size <= 128 * 8) TL_NORM_BW(128, 8, 1, true);
+    else if (size <= 256 * 8) TL_NORM_BW(256, 8, 1, true);
+    else if (size <= 512 * 8) TL_NORM_BW(512, 8, 1, true);
+    else if (size <= 1024 * 8) TL_NORM_BW(1024, 8, 1, false);
+    else TL_NORM_BW(1024, 16, 1, false);
 #undef TL_NORM_BW
 }
 

@@ -113,3 +113,22 @@ for memory in (False, True):
         err, n = lib.trainlib_last_error(), fake.fake_launches()
         assert (err == pkg.TL_OK and n > 0) if memory else (err != pkg.TL_OK and n == 0), (memory, name, err, n)
 """)
+
+
+def test_norm_backward_without_a_status_word_is_an_error(on_fake_runtime):
+    """rows of up to 8192 that start on 16 bytes go through a ring of bulk copies, whose waits report: without the word for that nothing is launched.  Other
+    rows have no such waits and run."""
+    on_fake_runtime(r"""
+x = lib.trainlib_malloc(1 << 22)
+keep = pkg.Keep()
+for memory in (False, True):
+    fake.fake_no_memory_for(ctypes.c_size_t(0 if memory else 4))
+    for p in ("fp32", "fp16"):
+        for size in (8, 64, 256, 264, 512, 1000, 2048, 4096, 8192, 8200, 16384, 16392, 9, 511, 16383):
+            a = pkg.make_args(keep, "trainlib_rmsnorm_args", sum=x, weight=x, dy=x, dx=x, dweight=x, eps=1e-5, rows=16, size=size)
+            lib.trainlib_clear_error()
+            fake.fake_reset(0)
+            getattr(lib, "trainlib_rmsnorm_%s_bw_cl" % p)(ctypes.byref(a))
+            err, n = lib.trainlib_last_error(), fake.fake_launches()
+            assert (err == pkg.TL_OK and n >= 2) if memory or size > 8192 or size % 8 else (err != pkg.TL_OK and n == 0), (memory, p, size, err, n)
+""")
