@@ -143,7 +143,8 @@ void  trainlib_rmsnorm_fp16_bw_cl(void *trainlib_rmsnorm_args);
  * The product silu(gate) * up and its gradients are library scratch of `rows * hidden` elements each (`hidden` rounded up to 128
  * bytes): three of them in the backward pass; beside them copies of operands whose rows do not start on 16 bytes, in fp32 of every
  * operand twice, and partial sums of up to 64 MB a gradient.  In fp16 silu(gate) * up and the gradients are rounded to fp16 between the products
- * (what passes 65504 there is infinite); up to eight rows of a forward pass it goes on unrounded.  A call repeated gives the same bits;
+ * (what passes 65504 there is infinite); up to eight rows of a forward pass it goes on as two halves, itself and what its rounding left: to 22 bits or
+ * 2^-25, infinite beyond 65504 all the same.  A call repeated gives the same bits;
  * rows, alignment and which gradients are asked for together may change the order of a sum.  Outputs must not overlap inputs or
  * each other. */
 struct trainlib_gated_ffn_args {

@@ -740,3 +740,28 @@ def test_norm_weights_that_are_no_numbers(ops, size, dt):
                 assert not torch.isfinite(scale).any(), (what, at)
                 assert (q[:, at] == 0).all(), (what, at)
                 assert torch.equal(total, clean)
+
+
+@pytest.mark.parametrize("h", [16, 40, 258, 1026, 2730, 4096])
+@pytest.mark.parametrize("rows", [1, 2, 5, 8])
+def test_ffn_few_halves_pass_the_gated_product_on_in_two_parts(ops, rows, h):
+    """Up to eight tokens in half precision silu(gate) * up reaches the second product as itself and what its rounding left.  Seen where results cancel:
+    columns 2 j and 2 j + 1 have the same gate and ups whose quotient is 1 + 2^-10, and result j is their difference, 2^-10 H.  H rounded once would
+    be off by up to half of that; in two parts what counts, relative to H, is: 2^-22 of either column (the second part's rounding), n + 1 roundings
+    or cuts of 2^-23 in either up and its product with silu(gate) (the gates are the same bits), and 2^-22 at each of the four terms that the sum adds."""
+    dt, n = torch.float16, 8
+    m = h // 2
+    x = (1 + randn(140, rows, n).abs().clamp(max=1)).to(dt)
+    wg = (randn(141, m, n).abs() / n).to(dt).repeat_interleave(2, 0)
+    wu = torch.ones(h, n, device="cuda", dtype=dt)
+    wu[1::2] = 1 + 2.0 ** -10
+    wd = torch.zeros(m, h, device="cuda", dtype=dt)
+    at = torch.arange(m, device="cuda")
+    wd[at, 2 * at], wd[at, 2 * at + 1] = -1, 1
+    gd, ud = x.double() @ wg.double().T, x.double() @ wu.double().T
+    hd = silu(gd) * ud
+    want, size = hd @ wd.double().T, hd[:, 1::2]
+    for shift in (0, 1):
+        y = blank(rows, m, dt=dt, shift=shift)
+        ops.ffn_fw(*[blank(*t.shape, dt=dt, shift=shift).copy_(t) for t in (x, wg, wu, wd)], None, None, y)
+        within(y, want, want.abs() * (HALF[dt] + 2.0 ** -16) + size * (2 * 2.0 ** -22 + 2 * (n + 1) * 2.0 ** -23 + 4 * 2.0 ** -22), "y")
