@@ -103,7 +103,7 @@ class State(object):
     """A program's tensors and, once the library has been called, its argument structs."""
 
     def __init__(self, case):
-        self.case, self.calls = case, None
+        self.case, self.calls, self.stream = case, None, 0
 
 
 def _randn(gen, *shape, scale=1.0, dtype=torch.float32):
@@ -221,6 +221,8 @@ def _int8(s):
 
 # ------------------------------------------------------------------------------------------------ the framework's kernels
 _pkg = None
+_on = None                                                    # the stream that the library's calls are queued on
+LEGACY = 1                                                    # CUDA's handle of the default stream, which torch gives as 0
 
 
 def _library():
@@ -238,6 +240,7 @@ def _own_calls(s):
     pkg, lib = _library()
     c, p = s.case, s.case["dtype"]
     s.keep = pkg.Keep()
+    s.stream = torch.cuda.current_stream().cuda_stream or LEGACY
 
     def call(name, struct, **fields):
         at = {k: v.data_ptr() if isinstance(v, torch.Tensor) else v for k, v in fields.items()}
@@ -269,11 +272,18 @@ def _own_calls(s):
 
 
 def run(s):
+    global _on
     if own:
-        if s.calls is None:
+        first = s.calls is None
+        if first:
             s.calls = _own_calls(s)
+        if _on != s.stream:                                   # behind the kernels that made the inputs, in front of those that read what leaves
+            _on = s.stream
+            _library()[1].trainlib_set_stream(_on)
         for fn, args in s.calls:
             fn(args)
+        if first:
+            _pkg.check(_pkg.load())                           # a refused call left its outputs as they were
         return s.out
     return {"norm_fw": _norm_fw, "norm_bw": _norm_bw, "ffn_fw": _ffn_fw, "ffn_bw": _ffn_bw, "int8": _int8}[s.case["kind"]](s)
 
