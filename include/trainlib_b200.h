@@ -31,7 +31,8 @@ void        trainlib_clear_error(void);
  * so call order is execution order.  trainlib_init is implicit in every entry point. */
 int   trainlib_init(int device);              /* returns TL_OK or an error code */
 int   trainlib_device(void);
-void  trainlib_set_stream(void *cuda_stream); /* NULL = the library's own stream.  Library scratch is shared: what is queued on the new
+void  trainlib_set_stream(void *cuda_stream); /* NULL = the library's own stream, which no other stream waits for; CUDA's default stream is
+                                               * cudaStreamLegacy (where a framework gives its handle as 0).  Library scratch is shared: what is queued on the new
                                                * stream waits for the calls of the one before where both use it.  Pending deferred
                                                * sums run on the stream before: it must still exist. */
 void *trainlib_stream(void);

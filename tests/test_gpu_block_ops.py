@@ -765,3 +765,31 @@ def test_ffn_few_halves_pass_the_gated_product_on_in_two_parts(ops, rows, h):
         y = blank(rows, m, dt=dt, shift=shift)
         ops.ffn_fw(*[blank(*t.shape, dt=dt, shift=shift).copy_(t) for t in (x, wg, wu, wd)], None, None, y)
         within(y, want, want.abs() * (HALF[dt] + 2.0 ** -16) + size * (2 * 2.0 ** -22 + 2 * (n + 1) * 2.0 ** -23 + 4 * 2.0 ** -22), "y")
+
+
+@both
+def test_on_the_default_stream(ops, dt):
+    """cudaStreamLegacy, where torch's own kernels are queued: behind the one that makes the input and in front of the one that reads the result, without a
+    wait on the host; then the library's own stream again"""
+    rows, n, h = 90, 256, 384
+    x, wg, wu, wd = ffn_tensors(rows, n, h, n, dt)
+    w, y, y2, z, z2 = torch.ones(n, device="cuda", dtype=dt), blank(rows, n, dt=dt), blank(rows, n, dt=dt), blank(rows, n, dt=dt), blank(rows, n, dt=dt)
+    ops.norm_fw(x, None, w, None, z)
+    ops.ffn_fw(z, wg, wu, wd, None, None, y)
+    torch.cuda.synchronize()
+    assert torch.cuda.current_stream().cuda_stream == 0
+    ops.lib.trainlib_set_stream(1)
+    try:
+        for turn in range(3):
+            late = torch.zeros_like(x)
+            for _ in range(20):
+                late.copy_(x)
+            ops.norm_fw(late, None, w, None, z2, sync=False)
+            ops.ffn_fw(z2, wg, wu, wd, None, None, y2, sync=False)
+            got, norm = y2.clone(), z2.clone()
+            y2.zero_(), z2.zero_()
+            assert torch.equal(got, y) and torch.equal(norm, z), turn
+    finally:
+        torch.cuda.synchronize()
+        ops.lib.trainlib_set_stream(None)
+    ops.pkg.check(ops.lib)
