@@ -793,3 +793,172 @@ def test_on_the_default_stream(ops, dt):
         torch.cuda.synchronize()
         ops.lib.trainlib_set_stream(None)
     ops.pkg.check(ops.lib)
+
+
+# ------------------------------------------------------------------------------------------------ tensors whose elements' numbers pass 32 bits
+def filled(seed, *shape, dt=torch.float16, scale=1.0):
+    """seeded values without a copy in single precision"""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    if dt == torch.int8:
+        return torch.randint(-128, 128, shape, device="cuda", generator=gen, dtype=dt)
+    t = torch.empty(shape, device="cuda", dtype=dt).normal_(generator=gen)
+    return t.mul_(scale) if scale != 1 else t
+
+
+@pytest.mark.parametrize("rows,size", [(1048581, 2056), (1048581, 2051), (107401, 20008), (107401, 20003)])
+def test_norms_beyond_32_bits(ops, rows, size):
+    """more than 2^31 elements: rows in front of, at and behind that border, and the weight's gradient over all of them"""
+    dt = torch.float16
+    x, w = filled(150, rows, size), (1 + randn(151, size, scale=0.3)).to(dt)
+    assert x.numel() > 2 ** 31
+    at = torch.tensor([0, 2 ** 31 // size - 1, 2 ** 31 // size, 2 ** 31 // size + 1, rows - 2, rows - 1], device="cuda")
+    h = x[at].double()
+    want, r = norm_ref(h, w.double())
+    y, q, scale = torch.empty_like(x), torch.empty(rows, size, dtype=torch.int8, device="cuda"), blank(rows)
+    ops.norm_fw(x, None, w, None, y)
+    within(y[at], want, want.abs() * (HALF[dt] + (size / 64 + 16) * U) + TINY[dt], "norm")
+    for call, v in ((lambda: ops.norm_int8(x, None, w, None, q, scale), want), (lambda: ops.rows_int8(x, q, scale), h)):
+        call()
+        step = v.abs().amax(1) / 127
+        within(scale[at], step, step * (size / 64 + 16) * U, "scale")
+        within(q[at], v / step[:, None], 0.5 + 127 * 8 * U, "q")
+    del q, scale
+    # backward, dy = the norm's result and a fraction of it, the gradient over it.  The sum over the rows of dy h r is the sum of w (h r)^2, about w times
+    # `rows`, in the first pass: beyond 65504 and half a step (65520) that is infinite in half precision.
+    for fraction in (1, 2.0 ** -10):
+        ops.norm_fw(x, None, w, None, y)
+        y.mul_(fraction)
+        dy, dw = y[at].double(), blank(size, dt=dt)
+        want_dw, terms = torch.zeros(size, device="cuda", dtype=torch.float64), torch.zeros(size, device="cuda", dtype=torch.float64)
+        for k in range(0, rows, 65536):
+            hk = x[k:k + 65536].double()
+            p = y[k:k + 65536].double() * hk / ((hk * hk).mean(1, keepdim=True) + EPS).sqrt()
+            want_dw += p.sum(0)
+            terms += p.abs().sum(0)
+        del hk, p
+        ops.norm_bw(x, w, y, None, y, dw)
+        g = dy * w.double()
+        want = r * (g - h * r * r * (g * h).mean(1, keepdim=True))
+        parts = r * g.abs() + h.abs() * r ** 3 * (g * h).abs().mean(1, keepdim=True)
+        within(y[at], want, want.abs() * HALF[dt] + parts * (size / 64 + 16) * U + TINY[dt], "dx")
+        off = terms * (rows / 32 + size / 64 + 128) * U
+        over, fits = want_dw.abs() - off >= 65520, want_dw.abs() + off < 65520
+        assert torch.isinf(dw[over]).all() and (fits.all() or fraction == 1)
+        if fits.any():
+            within(dw[fits], want_dw[fits], (want_dw.abs() * HALF[dt] + off + TINY[dt])[fits], "dweight")
+
+
+@pytest.mark.parametrize("rows", [2, 20, 40])
+@pytest.mark.parametrize("n,h", [(8200, 262147), (8193, 262200)])
+def test_ffn_weights_beyond_32_bits(ops, rows, n, h):
+    """weights of more than 2^31 elements; only the last hidden columns reach the result and the gradients"""
+    dt, m, live = torch.float16, 24, 64
+    x, wg, wu = randn(152, rows, n, dt=dt), filled(153, h, n, scale=n ** -0.5), filled(154, h, n, scale=n ** -0.5)
+    assert wg.numel() > 2 ** 31
+    wd = torch.zeros(m, h, device="cuda", dtype=dt)
+    wd[:, h - live:] = randn(155, m, live, scale=live ** -0.5)
+    gd, ud = x.double() @ wg[h - live:].double().T, x.double() @ wu[h - live:].double().T
+    tail = wd[:, h - live:].double()
+    y, g, u = blank(rows, m, dt=dt), blank(rows, h, dt=dt), blank(rows, h, dt=dt)
+    ops.ffn_fw(x, wg, wu, wd, g, u, y)
+    near(g[:, h - live:], gd, dt, 1, (n,), "gate")
+    near(u[:, h - live:], ud, dt, 1, (n,), "up")
+    near(y, (silu(gd) * ud) @ tail.T, dt, 2, (3 * n, h), "y", (silu(gd) * ud).square() @ tail.square().T)
+    dy, dx, dwu, dwd = randn(156, rows, m, dt=dt), blank(rows, n, dt=dt), torch.empty_like(wu), blank(m, h, dt=dt)
+    ops.ffn_bw(x, wg, wu, wd, g, u, dy, dx, None, dwu, dwd)
+    want, terms = ffn_bw_ref(x, wg[h - live:], wu[h - live:], wd[:, h - live:], g[:, h - live:], u[:, h - live:], dy)
+    near(dx, want[0], dt, 2, (m, 2 * h), "dx", terms[0])
+    near(dwu[h - live:], want[2], dt, 2, (m, rows), "dw_up", terms[2])
+    near(dwd[:, h - live:], want[3], dt, 2, (m, rows), "dw_down", terms[3])
+    assert (dwu[:h - live].amax(1) == 0).all() and (dwu[:h - live].amin(1) == 0).all()
+
+
+@pytest.mark.parametrize("h", [32776, 32771])
+def test_ffn_tokens_beyond_32_bits(ops, h):
+    """projections of more than 2^31 elements"""
+    dt, rows, n, m, live = torch.float16, 65600, 72, 40, 128
+    x, wg, wu, wd = ffn_tensors(rows, n, h, m, dt)
+    y, g, u = blank(rows, m, dt=dt), torch.empty(rows, h, device="cuda", dtype=dt), torch.empty(rows, h, device="cuda", dtype=dt)
+    assert g.numel() > 2 ** 31
+    ops.ffn_fw(x, wg, wu, wd, g, u, y)
+    gd, ud = x[-live:].double() @ wg.double().T, x[-live:].double() @ wu.double().T
+    near(g[-live:], gd, dt, 1, (n,), "gate")
+    near(u[-live:], ud, dt, 1, (n,), "up")
+    near(y[-live:], (silu(gd) * ud) @ wd.double().T, dt, 2, (3 * n, h), "y", (silu(gd) * ud).square() @ wd.double().square().T)
+    del gd, ud
+    dy = randn(157, rows, m, dt=dt)
+    got = [blank(*t.shape, dt=dt) for t in (x, wg, wu, wd)]
+    ops.ffn_bw(x, wg, wu, wd, g, u, dy, *got)
+    want, terms = ffn_bw_ref(x[-live:], wg, wu, wd, g[-live:], u[-live:], dy[-live:])
+    near(got[0][-live:], want[0], dt, 2, (m, 2 * h), "dx", terms[0])
+    want, terms = ffn_bw_ref(x, wg[-live:], wu[-live:], wd[:, -live:], g[:, -live:], u[:, -live:], dy)
+    for k, (t, v, q, what) in enumerate(zip(got, want, terms, ("dx", "dw_gate", "dw_up", "dw_down"))):
+        if k:
+            near(t[:, -live:] if k == 3 else t[-live:], v, dt, 2, (m, rows), what, q)
+
+
+@pytest.mark.parametrize("rows", [2, 20, 40])
+@pytest.mark.parametrize("n", [32016, 32007])
+def test_linear_in_8_bits_beyond_32_bits(ops, rows, n):
+    m, live = 70001, 40
+    x, w = filled(158, rows, n, dt=torch.int8), filled(159, m, n, dt=torch.int8)
+    assert w.numel() > 2 ** 31
+    y = blank(rows, m)
+    ops.linear_int8(x, torch.ones(rows, device="cuda"), w, torch.ones(m, device="cuda"), None, y)
+    for cols in (slice(0, live), slice(2 ** 31 // n - live // 2, 2 ** 31 // n + live // 2), slice(m - live, m)):
+        assert torch.equal(y[:, cols], (x.double() @ w[cols].double().T).float())
+
+
+@both
+@pytest.mark.parametrize("rows", [6, 70])
+def test_alternating_between_streams(ops, rows, dt):
+    """two streams of the caller in turn: the scratch that their calls share passes from one to the other, and each result is its own"""
+    n, h = 260, 1000
+    progs = []
+    for k in range(2):
+        x, wg, wu, wd = ffn_tensors(rows, n, h, n, dt, seed=160 + 10 * k)
+        y, g, u = blank(rows, n, dt=dt), blank(rows, h, dt=dt), blank(rows, h, dt=dt)
+        dy, w = randn(165 + 10 * k, rows, n, dt=dt), (1 + randn(166 + 10 * k, n, scale=0.2)).to(dt)
+        grads = [blank(*t.shape, dt=dt) for t in (x, wg, wu, wd)] + [blank(rows, n, dt=dt), blank(n, dt=dt)]
+
+        def step(x=x, ws=(wg, wu, wd), y=y, g=g, u=u, dy=dy, w=w, grads=grads):
+            ops.ffn_fw(x, *ws, g, u, y, sync=False)
+            ops.ffn_bw(x, *ws, g, u, dy, *grads[:4], sync=False)
+            ops.norm_bw(y, w, grads[0], dy, grads[4], grads[5], sync=False)
+        torch.cuda.synchronize()
+        step()
+        ops.lib.trainlib_synchronize()
+        outs = [y, g, u] + grads
+        progs.append((step, outs, [t.clone() for t in outs]))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(8):
+        for _, outs, _ in progs:
+            for t in outs:
+                t.fill_(3)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for s, (step, _, _) in zip(streams, progs):
+                ops.lib.trainlib_set_stream(s.cuda_stream)
+                step()
+        torch.cuda.synchronize()
+        for _, outs, first in progs:
+            assert all(torch.equal(a, b) for a, b in zip(outs, first)), turn
+    ops.lib.trainlib_set_stream(None)
+    ops.pkg.check(ops.lib)
+
+
+@both
+@pytest.mark.parametrize("rows,n,h,m", [(7, 72, 200, 40), (65, 130, 257, 63), (300, 264, 520, 136)])
+def test_ffn_gradients_in_every_combination(ops, rows, n, h, m, dt):
+    """each set of wanted gradients, and nothing written for the others"""
+    x, wg, wu, wd = ffn_tensors(rows, n, h, m, dt)
+    g, u, dy = randn(170, rows, h, dt=dt), randn(171, rows, h, dt=dt), randn(172, rows, m, dt=dt)
+    want, terms = ffn_bw_ref(x, wg, wu, wd, g, u, dy)
+    for mask in range(1, 16):
+        got = [blank(*t.shape, dt=dt) for t in (x, wg, wu, wd)]
+        ops.ffn_bw(x, wg, wu, wd, g, u, dy, *[t if mask >> k & 1 else None for k, t in enumerate(got)])
+        for k, (t, v, q, l) in enumerate(zip(got, want, terms, (2 * h, rows, rows, rows))):
+            if mask >> k & 1:
+                near(t, v, dt, 2, (m, l), (mask, k), q)
+            else:
+                assert (t == 77).all()
