@@ -120,7 +120,8 @@ void  trainlib_gelu_fp16_bw_cl(void *act_args_fp16);
  *          dx = dsum + r * (g - h * r^2 * mean(g * h)) is the gradient of x and of residual; dsum (NULL: none) is the gradient that
  *          reaches the sum along the residual path.  dweight[j] = sum over the rows of dy * h * r.  dx or dweight may be NULL (not
  *          wanted), not both.  dx may be dy, dsum or sum itself.
- * The sum of a row's squares is a float: where it overflows, r is 0 (results of 0, in 8 bits a scale that is NaN).
+ * The sum of a row's squares is a float: where it overflows, r is 0 (results of 0, in 8 bits a scale that is NaN); squares below 2^-126, which count only
+ * where eps is as small, lose their digits.
  * Every row is reduced in one fixed order and so are the rows of dweight: a call repeated gives the same bits (the order depends on
  * the sizes and on whether all tensors start on 16 bytes). */
 struct trainlib_rmsnorm_args {
@@ -146,8 +147,9 @@ void  trainlib_rmsnorm_fp16_bw_cl(void *trainlib_rmsnorm_args);
  * operand twice, and partial sums of up to 64 MB a gradient.  In fp16 silu(gate) * up and the gradients are rounded to fp16 between the products
  * (what passes 65504 there is infinite); up to eight rows of a forward pass it goes on as two halves, itself and what its rounding left: to 22 bits or
  * 2^-25, infinite beyond 65504 all the same.  A call repeated gives the same bits;
- * rows, alignment and which gradients are asked for together may change the order of a sum.  Outputs must not overlap inputs or
- * each other. */
+ * rows, alignment and which gradients are asked for together may change the order of a sum.  In fp32 the products take every operand as two parts
+ * (a forward pass of up to four rows does not): an infinite operand gives NaN there, and so does one from 2^128 - 2^116 on, whose first part is infinite.
+ * Outputs must not overlap inputs or each other. */
 struct trainlib_gated_ffn_args {
     void *x; void *w_gate; void *w_up; void *w_down; void *gate; void *up; void *y;
     int rows; int in_size; int hidden; int out_size;

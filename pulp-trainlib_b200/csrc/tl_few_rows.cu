@@ -303,8 +303,11 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) few_rows_kernel(const 
     }
 }
 
-// Single precision, up to four tokens, on FFMA: R rows of each matrix per CTA, its warps share K, lanes along it.  V: elements per load.  (One token, 1024 x 2048 x
-// 1024: 6.4 us, on the tensor cores 9.8; rows of odd length 7.9 and 21.6.  Eight tokens: 20.7 and 10.2.)
+// Single precision, up to four tokens, on FFMA: R rows of each matrix per CTA, its warps share K, lanes along it.  V: elements per load.  Whole blocks, both products,
+// weights from memory, FFMA against the tensor cores in us:  one token 3.4 / 5.1 (512 x 512 x 512), 8.6 / 11.0 (1024 x 2048 x 1024), 12.5 / 19.1 (1000 x 2731 x 1000),
+// 32.2 / 37.9 (2048 x 5632 x 2048), 44.4 / 44.7 (4096 x 4096 x 4096).  Two to four tokens, which cost the same: 4.0 / 5.3, 12.6 / 11.1, 21.7 / 19.2, 51.8 / 38.1,
+// 62.0 / 44.5, and 7.0 / 9.9 (257 x 1001 x 257), 10.6 / 10.3 (640 x 1712 x 640), 15.5 / 16.3 (1000 x 2736 x 1000): the bound of four is right for weights of up to
+// some 10 MB that fit a wave or two of CTAs, and too high for larger ones by up to 1.4 times.
 template <int EPI, int NT, int R, int V>
 __global__ void __launch_bounds__(256) few_rows_fp32_kernel(const __grid_constant__ FewParams<float> p)
 {

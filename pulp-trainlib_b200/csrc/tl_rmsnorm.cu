@@ -391,7 +391,8 @@ template <class T> static int ring_stages(int groups, int in, int size) { return
 // ---------------------------------------------------------------- forward
 // G threads per row, a block's rows side by side, NV packs of V elements per thread; small CTAs, so that one's loads cover the other's stores.  Measured with
 // x, residual, sum and y of 2^25 elements (41 us half, 82 us single at the rate of a plain copy): halves 40.4 us at 256 columns, 40.8 at 1000 and 2048, 41.4 at 8192,
-// 44.8 at 16384; floats 79 us from 256 to 8192 columns, 84 at 16384; 999 columns, element by element, 58 and 80 us.
+// 44.8 at 16384; floats 79 us from 256 to 8192 columns, 84 at 16384; 999 columns, element by element, 58 and 80 us.  To 8 bits, with the sum: 41.7 and 40.7 us
+// for halves at 2048 and 8192 columns (35.9), 75 at 999; 32.9 for 2^24 floats at 2048 (33.3).
 // (CTAs per SM that the registers are held down to: 1024 threads with 4 or 8 packs each, 768 of 256 with 8, 1280 with fewer)
 constexpr int fw_blocks(int g, int nv, bool few) { return g < 512 ? nv == 8 ? 3 : nv == 4 ? 4 : 5 : nv == 4 || few ? 2 : 1; }
 template <class T, int MODE, int G, int NV, int V>
@@ -518,7 +519,8 @@ __global__ void __launch_bounds__(1024) rmsnorm_fw_wide_kernel(const T *x, const
 }
 
 // The 8-bit form of half-precision rows as they are: a CTA of G threads per row, the halves in registers as they lie, the largest magnitude two at a time.
-// 4096 rows of 8192: 32 us (a ring in shared memory with one CTA per SM: 35), the bytes alone 15; the rounding's fourteen instructions per element hold it there.
+// 4096 rows of 8192: 26 us, the bytes alone 15; the rounding's fourteen instructions per element hold it there.  (A ring in shared memory with one CTA per SM was a tenth
+// slower; a second division in quant_exact made it 29: most rows have a value near a border.)
 template <int G, int NV>
 __global__ void __launch_bounds__(G, 1280 / G) quantize_rows_kernel(const __half *__restrict__ x, signed char *__restrict__ q, float *__restrict__ scale, int size)
 {
